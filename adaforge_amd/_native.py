@@ -17,6 +17,10 @@ AF_ERR_NO_DEVICE = 5
 AF_MAX_CONTEXT = 32768
 AF_MAX_NEW_TOKENS = 128
 AF_LAYER_V_NORM = 1
+AF_KV_F16, AF_KV_Q4 = 0, 1
+AF_MAX_SEQUENCES, AF_MAX_BATCH_TOKENS, AF_MAX_HEADS, AF_MAX_POSITIONS = 65535, 65536, 1024, 1 << 24
+AF_NO_TOKEN = 0xFFFFFFFF
+AF_MAX_LOGIT_ROWS, AF_MAX_HISTORY = 16384, 65535
 
 P = ctypes.c_void_p
 u8p = ctypes.POINTER(ctypes.c_uint8)
@@ -66,6 +70,33 @@ class AttentionArgs(ctypes.Structure):
     _fields_ = [("q", P), ("k", P), ("v", P), ("q_norm", P), ("k_norm", P), ("q_eps", f32), ("k_eps", f32),
                 ("v_eps", f32), ("v_norm", i32), ("rope", RopeDesc), ("config", AttentionConfigDesc),
                 ("k_cache", P), ("v_cache", P), ("ring", u32), ("position", u32), ("out", P)]
+
+
+class KvPages(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("type", u32), ("pages", u32), ("page", u32), ("kv_heads", u32), ("width", u32)]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("starts", P), ("lengths", P), ("table", P), ("table_stride", u32), ("sequences", u32), ("tokens", u32)]
+
+
+class KvAppendArgs(ctypes.Structure):
+    _fields_ = [("q", P), ("q_stride", u32), ("k", P), ("k_stride", u32), ("v", P), ("v_stride", u32), ("q_norm", P),
+                ("k_norm", P), ("q_eps", f32), ("k_eps", f32), ("v_eps", f32), ("v_norm", i32), ("rope", P),
+                ("q_heads", u32), ("q_out", P), ("q_out_stride", u32), ("pages", KvPages), ("batch", KvBatch)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [("q", P), ("q_stride", u32), ("out", P), ("out_stride", u32), ("config", AttentionConfigDesc),
+                ("sinks", u32), ("pages", KvPages), ("batch", KvBatch), ("longest_query", u32), ("longest_context", u32),
+                ("workspace", P)]
+
+
+class LogitsArgs(ctypes.Structure):
+    _fields_ = [("logits", P), ("stride", u32), ("out", P), ("out_stride", u32), ("rows", u32), ("vocabulary", u32),
+                ("penalties", P), ("history", P), ("history_stride", u32), ("history_len", P), ("bias_ids", P),
+                ("bias_values", P), ("bias_stride", u32), ("bias_len", P), ("mask", P), ("mask_stride", u32),
+                ("result", P), ("workspace", P)]
 
 
 class LayerDesc(ctypes.Structure):
@@ -126,6 +157,17 @@ SIGNATURES = {
     "af_ffn_free": (None, [P]),
     "af_ffn_run": (i32, [P, P, P, P]),
     "af_attention_decode": (i32, [ctypes.POINTER(AttentionArgs), P]),
+    "af_workspace_create": (i32, [sz, ctypes.POINTER(P)]),
+    "af_workspace_free": (None, [P]),
+    "af_rope_create": (i32, [ctypes.POINTER(RopeDesc), ctypes.POINTER(P)]),
+    "af_rope_free": (None, [P]),
+    "af_kv_page_bytes": (sz, [u32, u32, u32, u32]),
+    "af_kv_append": (i32, [ctypes.POINTER(KvAppendArgs), P]),
+    "af_kv_read": (i32, [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch), P, P, P]),
+    "af_paged_attention": (i32, [ctypes.POINTER(PagedAttentionArgs), P]),
+    "af_paged_attention_workspace": (i32, [ctypes.POINTER(PagedAttentionArgs), ctypes.POINTER(sz)]),
+    "af_logits_select": (i32, [ctypes.POINTER(LogitsArgs), P]),
+    "af_logits_select_workspace": (i32, [ctypes.POINTER(LogitsArgs), ctypes.POINTER(sz)]),
     "af_session_open": (i32, [ctypes.POINTER(LayerDesc), u32, ctypes.POINTER(HeadDesc), u32, ctypes.POINTER(P)]),
     "af_session_generate": (i32, [P, u32p, sz, u32p, sz, u32, TOKEN_FN, P, u32p, ctypes.POINTER(sz),
                                   ctypes.POINTER(i32), ctypes.POINTER(GenerationStats)]),

@@ -1,0 +1,148 @@
+// The paged KV cache of several sequences: where a batch's tokens stand, which keys they see, and the kernels'
+// arguments.  The index arithmetic compiles for the host too (tests run it there); device arrays may hold anything,
+// so every value read from one is cut to range here.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#include <hip/hip_runtime.h>
+#define AF_HD __host__ __device__ __forceinline__
+#else
+#define AF_HD inline
+#endif
+
+namespace af {
+
+struct PagedBatch {
+    const uint32_t* starts;
+    const uint32_t* lengths;
+    const uint32_t* table;
+    uint32_t table_stride, sequences, tokens;
+    uint32_t pages, page_shift;  // pages of 2^page_shift tokens
+};
+
+constexpr int32_t kNoPosition = -(1 << 30);
+
+// A sequence's rows [first, first + count) of the batch, the position of the first, and the keys [0, end) that its
+// table can hold.
+struct Span {
+    uint32_t first, count;
+    int32_t pos0;
+    uint32_t end;
+};
+
+AF_HD Span span_of(uint32_t start, uint32_t stop, uint32_t length, const PagedBatch& b) {
+    const uint32_t len = length < (1u << 30) ? length : 1u << 30;
+    const uint32_t a = start < b.tokens ? start : b.tokens, e = stop < b.tokens ? stop : b.tokens;
+    const uint32_t cap = b.table_stride << b.page_shift;  // (at most 2^24: checked by the call)
+    Span s;
+    s.first = a;
+    s.count = e > a ? e - a : 0;
+    const int64_t p = (int64_t)len - ((int64_t)stop - (int64_t)a);
+    s.pos0 = s.count && p > kNoPosition ? (int32_t)p : kNoPosition;
+    s.end = len < cap ? len : cap;
+    return s;
+}
+
+// Whether the query at position p sees key j (of those its sequence holds).
+AF_HD bool sees(int32_t p, int32_t j, uint32_t window, uint32_t sinks) {
+    return j <= p && (window == 0 || (uint32_t)(p - j) < window || (uint32_t)j < sinks);
+}
+
+// The key tiles (of T keys) that hold every key seen by queries at positions plo .. phi: tiles [0, head), then from,
+// from + 1, ...; `count` in all.
+struct Tiles {
+    uint32_t head, from, count;
+};
+
+template <uint32_t T>
+AF_HD Tiles tiles_of(int32_t plo, int32_t phi, uint32_t end, uint32_t window, uint32_t sinks) {
+    Tiles t = {0, 0, 0};
+    if (phi < 0) return t;
+    const uint32_t hi = (uint32_t)phi + 1 < end ? (uint32_t)phi + 1 : end;  // keys [0, hi)
+    const uint32_t low = plo < 0 ? 0u : (uint32_t)plo;
+    const uint32_t lo = window != 0 && low + 1 > window ? low + 1 - window : 0u;
+    const uint32_t to = (hi + T - 1) / T;
+    uint32_t first = sinks < lo ? sinks : lo;  // first tokens that the window leaves out
+    t.head = (first + T - 1) / T;
+    if (t.head > to) t.head = to;
+    t.from = lo / T > t.head ? lo / T : t.head;
+    t.count = t.head + (to > t.from ? to - t.from : 0);
+    return t;
+}
+
+AF_HD uint32_t tile_at(const Tiles& t, uint32_t i) { return i < t.head ? i : t.from + (i - t.head); }
+
+// Bytes of one KV head's part of a page.
+AF_HD uint32_t page_part_bytes(bool q4, uint32_t page, uint32_t width) {
+    return q4 ? page * (width / 16 * 9) : page * width * 2;
+}
+
+#ifdef __HIPCC__
+
+struct KvAppend {
+    const float *q, *k, *v;
+    uint32_t q_stride, k_stride, v_stride;
+    const float *q_norm, *k_norm;
+    float q_eps, k_eps, v_eps;
+    uint32_t v_norm;
+    const uint64_t* turns;  // per pair, the fraction of a turn per position (null: no rotation)
+    uint32_t q_heads, kv_heads;
+    float* q_out;
+    uint32_t q_out_stride;
+    uint8_t *k_pages, *v_pages;
+    PagedBatch b;
+};
+hipError_t launch_kv_append(const KvAppend& a, uint32_t width, bool q4, hipStream_t s);
+hipError_t launch_kv_read(const uint8_t* k_pages, const uint8_t* v_pages, const PagedBatch& b, uint32_t kv_heads,
+                          uint32_t width, bool q4, uint16_t* k, uint16_t* v, hipStream_t s);
+
+struct PagedAttn {
+    const float* q;
+    float* out;
+    uint32_t q_stride, out_stride;
+    const uint8_t *k_pages, *v_pages;
+    uint32_t kv_heads, group;  // query heads per KV head
+    uint32_t window, sinks;
+    float scale;
+    PagedBatch b;
+    uint32_t* tickets;
+    float* part;
+};
+hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, hipStream_t s);
+
+struct LogitsSelect {
+    const float* logits;
+    float* out;
+    uint32_t stride, out_stride, rows, vocabulary;
+    const float* penalties;
+    const uint32_t *history, *history_len;
+    uint32_t history_stride;
+    const uint32_t* bias_ids;
+    const float* bias_values;
+    const uint32_t* bias_len;
+    uint32_t bias_stride;
+    const uint32_t* mask;
+    uint32_t mask_stride;
+    uint32_t* result;
+    uint32_t* tickets;
+    uint4* part;  // one (key high, key low, bad, 0) per slice of a row
+    uint32_t slice, slices;
+};
+hipError_t launch_logits_select(const LogitsSelect& a, hipStream_t s);
+
+#endif
+
+// A workspace starts with completion tickets, zero between calls; partial results follow.
+constexpr uint32_t kTickets = 16384;
+constexpr size_t kTicketBytes = kTickets * 4;
+
+// Tokens of a row's slice in the choice of a token, and the slices of a row.
+AF_HD uint32_t logits_slice(uint32_t rows, uint32_t vocabulary) {
+    (void)rows;
+    (void)vocabulary;
+    return 4096;
+}
+
+}  // namespace af

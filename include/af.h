@@ -196,6 +196,157 @@ typedef struct {
 } af_attention_args;
 int af_attention_decode(const af_attention_args* args, void* stream);
 
+/* ---- several sequences: a paged KV cache, attention over it, the choice of a token ---------------
+ *      (no counterpart in the reference, which decodes one sequence over contiguous buffers) --------- */
+
+/* Device memory that calls use between their launches' blocks: completion tickets (zero between calls) and
+ * partial results.  A call checks that its workspace is large enough (the *_workspace functions say how large:
+ * any call of the same sizes or smaller ones fits, of either kind) and on its stream's device.  Calls that share
+ * one must not overlap: give each stream, and each captured graph that may run beside another, its own.  It
+ * lives on the device current when it is created and must outlive the graphs captured with it. */
+typedef struct af_workspace af_workspace;
+int af_workspace_create(size_t bytes, af_workspace** out);
+void af_workspace_free(af_workspace* w);
+
+/* RoPE frequencies resident on the current device (validated as af_rope_params elsewhere; the context is
+ * not checked against positions that are in device memory).  Held as 64-bit fractions of a turn, so an angle is
+ * exact to 2^-64 turns per position. */
+typedef struct af_rope af_rope;
+int af_rope_create(const af_rope_params* params, af_rope** out);
+void af_rope_free(af_rope* r);
+
+/* A pool of pages, each `page` tokens of K (V alike) of every KV head: [kv_heads] parts of a page, and in a part
+ *   AF_KV_F16: fp16 [page][width];
+ *   AF_KV_Q4:  codes [page][width / 2 bytes], then scales fp16 [page][width / 32].
+ * A 4-bit block of 32 values has the scale d = fp16(m / -8), m its value of largest magnitude (the positive one of
+ * two), and codes n = rint(x / d) + 8 in 0..15 that stand for the fp16 value nearest d (n - 8).  Eight codes make a
+ * 32-bit word: values 2 i and 2 i + 1 at bits 4 i and 16 + 4 i.  A block with an infinity, a NaN or a scale
+ * beyond fp16 stands for NaNs.  `page` is 16, 32, 64, 128 or 256; width 64, 128, 256 or 512; k and v 16-byte aligned. */
+#define AF_KV_F16 0u
+#define AF_KV_Q4 1u
+typedef struct {
+    void* k; /* device, pages * af_kv_page_bytes */
+    void* v;
+    uint32_t type;
+    uint32_t pages;
+    uint32_t page;
+    uint32_t kv_heads;
+    uint32_t width;
+} af_kv_pages;
+/* Bytes of one page of K (V alike); 0 for a layout that is not supported. */
+size_t af_kv_page_bytes(uint32_t type, uint32_t page, uint32_t kv_heads, uint32_t width);
+
+/* A batch of new tokens: sequence s has rows starts[s] .. starts[s + 1] - 1 of the batch, its last positions: row
+ * starts[s + 1] - 1 is position lengths[s] - 1.  Position p lies in page table[s][p / page], slot p % page.  The
+ * arrays are device memory, read when the call runs (a captured call follows their later values): the call keeps
+ * every access in bounds whatever they hold.  A position without a page (a table entry that is not below
+ * `pages`, a position at or past table_stride * page, a negative one where lengths[s] is less than the sequence's
+ * rows) is not written and not seen, and reads as zeros; rows at or past starts[sequences] are left as they were.
+ * starts rises from 0 to at most `tokens` (later rows of a larger start are cut off). */
+typedef struct {
+    const uint32_t* starts;  /* device [sequences + 1] */
+    const uint32_t* lengths; /* device [sequences]: positions cached, the batch's included */
+    const uint32_t* table;   /* device [sequences][table_stride] page numbers */
+    uint32_t table_stride;
+    uint32_t sequences;      /* 1 to AF_MAX_SEQUENCES */
+    uint32_t tokens;         /* rows of the batch, 1 to AF_MAX_BATCH_TOKENS */
+} af_kv_batch;
+#define AF_MAX_SEQUENCES 65535u
+#define AF_MAX_BATCH_TOKENS 65536u
+#define AF_MAX_HEADS 1024u
+#define AF_MAX_POSITIONS 16777216u /* table_stride * page at most */
+
+/* What af_attention_decode does before it attends, for a batch: per-head RMSNorm of q and k (q_norm, k_norm
+ * NULL: none) and of v (v_norm, unit weights), NeoX RoPE of q and k at their positions (rope NULL: none), K and V
+ * appended, the queries written to q_out.  The products are 64-bit, rounded once to f32, then to the cache's type.
+ * Rows are [heads][width] floats, *_stride floats apart (multiples of 4; pointers 16-byte aligned).  q NULL: K and V
+ * only (q_heads 0).  q_out may be q itself with the same stride; no other output may overlap an input.  A
+ * page must not be named twice where both namings are written by the call. */
+typedef struct {
+    const float* q; /* device [tokens], as are k and v */
+    uint32_t q_stride;
+    const float* k;
+    uint32_t k_stride;
+    const float* v;
+    uint32_t v_stride;
+    const float* q_norm; /* device [width] */
+    const float* k_norm;
+    float q_eps, k_eps, v_eps;
+    int32_t v_norm;
+    const af_rope* rope;
+    uint32_t q_heads;
+    float* q_out;
+    uint32_t q_out_stride;
+    af_kv_pages pages;
+    af_kv_batch batch;
+} af_kv_append_args;
+int af_kv_append(const af_kv_append_args* args, void* stream);
+
+/* The fp16 values that the cache holds at the batch's positions: k and v (device) [tokens][kv_heads][width]. */
+int af_kv_read(const af_kv_pages* pages, const af_kv_batch* batch, uint16_t* k, uint16_t* v, void* stream);
+
+/* Causal attention of a batch over its sequences' pages, the new tokens' K and V among them: a query at
+ * position p sees every key j <= p of its sequence with window == 0, j > p - window, or j < sinks (the first
+ * tokens that stay visible).  out = softmax(scale q.k) v per query head (q_heads / kv_heads of them share a KV
+ * head), zeros where nothing is seen.  q as af_kv_append writes it; q and out rows are [q_heads][width] floats,
+ * strides and alignment as there, out not overlapping q.  fp32 softmax and sums; the queries and probabilities enter
+ * the products with at least 22 significant bits.  longest_query (new tokens) and longest_context (length) of any
+ * sequence are hints that only the split of the work, and the workspace's size, depend on: results are right
+ * whatever they are, but one sequence may get slow where they are too small. */
+typedef struct {
+    const float* q; /* device [tokens] */
+    uint32_t q_stride;
+    float* out;     /* device [tokens] */
+    uint32_t out_stride;
+    af_attention_config config;
+    uint32_t sinks;
+    af_kv_pages pages;
+    af_kv_batch batch;
+    uint32_t longest_query;
+    uint32_t longest_context;
+    af_workspace* workspace;
+} af_paged_attention_args;
+int af_paged_attention(const af_paged_attention_args* args, void* stream);
+/* Bytes of workspace for such a call (pointers in args are not looked at). */
+int af_paged_attention_workspace(const af_paged_attention_args* args, size_t* bytes);
+
+/* The logits of several sequences on the way to their next tokens.  For token t of row r, in 64 bits, rounded once:
+ *   y = logits[r][t];
+ *   t among the first history_len[r] ids of history[r], c times (c > 0):
+ *     y = (y > 0 ? y / repetition : y * repetition) - (frequency * c + presence);
+ *   t among the first bias_len[r] ids of bias_ids[r]: y += the last such bias;
+ *   bit t of mask[r] (word t / 32, bit t % 32) clear: y = -infinity, whatever it was.
+ * penalties (device [rows][3]: repetition, presence, frequency; NULL: none, as without history), biases
+ * and mask may be NULL.  Ids at or past the vocabulary are ignored; lengths above their stride count as the stride.
+ * out (NULL: not written; may be logits itself with its stride) gets y, result (device [rows][2]) the largest y's
+ * id (the smallest on ties; NaNs are passed over; AF_NO_TOKEN where every y is -infinity or NaN) and whether a NaN
+ * or +infinity is among the y.  Greedy as af_q6_gemv_argmax's result where nothing is given. */
+#define AF_NO_TOKEN 0xFFFFFFFFu
+#define AF_MAX_LOGIT_ROWS 16384u
+#define AF_MAX_HISTORY 65535u /* history_stride and bias_stride at most */
+typedef struct {
+    const float* logits; /* device [rows], stride floats apart */
+    uint32_t stride;
+    float* out;
+    uint32_t out_stride;
+    uint32_t rows;       /* 1 to AF_MAX_LOGIT_ROWS */
+    uint32_t vocabulary;
+    const float* penalties;
+    const uint32_t* history;     /* device [rows][history_stride] */
+    uint32_t history_stride;
+    const uint32_t* history_len; /* device [rows] */
+    const uint32_t* bias_ids;    /* device [rows][bias_stride] */
+    const float* bias_values;
+    uint32_t bias_stride;
+    const uint32_t* bias_len;
+    const uint32_t* mask;        /* device [rows][mask_stride] words */
+    uint32_t mask_stride;
+    uint32_t* result;
+    af_workspace* workspace;
+} af_logits_args;
+int af_logits_select(const af_logits_args* args, void* stream);
+int af_logits_select_workspace(const af_logits_args* args, size_t* bytes);
+
 /* ---- generation session: GpuDiagnostics::open_session / generate and GenerationSession
  *      (crates/application/src/lib.rs:29-47, 1092-1126; crates/cuda-backend/src/stack.rs:820-966,
  *      1146-1480) -------------------------------------------------------------------------- */
