@@ -79,6 +79,56 @@ AF_HD uint32_t page_part_bytes(bool q4, uint32_t page, uint32_t width) {
     return q4 ? page * (width / 16 * 9) : page * width * 2;
 }
 
+// A workspace starts with completion tickets, zero between calls; partial results follow.
+constexpr uint32_t kTickets = 16384;
+constexpr size_t kTicketBytes = kTickets * 4;
+
+// What the split of an attention call depends on: sizes, and the caller's hints.
+struct AttnShape {
+    uint32_t sequences, tokens, kv_heads, group, width, window, sinks;
+    uint32_t longest_query, longest_context, capacity;  // (capacity: positions a page table row holds)
+};
+
+// Row tiles' slots for partial sums: sequence s's tiles start at slot starts[s] group / R + s, so every sequence's lie
+// in front of the next one's whatever the starts are.
+AF_HD uint32_t row_slots(const AttnShape& a, uint32_t r) { return (uint32_t)((uint64_t)a.tokens * a.group / r) + a.sequences; }
+
+AF_HD uint32_t least(uint32_t a, uint32_t b) { return a < b ? a : b; }
+AF_HD uint32_t most(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// The longest key range of a row tile, in tiles of 32 keys, as the hints have it.
+AF_HD uint32_t longest_tiles(const AttnShape& a, uint32_t tokens) {
+    uint32_t keys = most(1, least(a.longest_context, a.capacity));
+    if (a.window) {
+        const uint64_t seen = (uint64_t)a.window + a.sinks + tokens + 64;
+        if (seen < keys) keys = (uint32_t)seen;
+    }
+    return (keys + 31) / 32;
+}
+
+// The launch over few rows: grid units (row tiles of 16, sequences, KV heads) by splits, each split a chunk of key tiles.
+struct FewPlan {
+    uint32_t row_tiles, splits, chunk;
+    size_t part_bytes;
+};
+
+AF_HD FewPlan few_plan(const AttnShape& a) {
+    FewPlan p;
+    const uint32_t tokens = most(1, least(a.longest_query, a.tokens));
+    const uint64_t pairs = (uint64_t)a.sequences * a.kv_heads;  // (at most 2^22: checked by the call)
+    p.row_tiles = (uint32_t)(((uint64_t)tokens * a.group + 15) / 16);
+    if (p.row_tiles * pairs > 1u << 22) p.row_tiles = most(1, (uint32_t)((1u << 22) / pairs));
+    const uint32_t units = (uint32_t)(p.row_tiles * pairs), tiles = longest_tiles(a, tokens);
+    const uint64_t slots = (uint64_t)row_slots(a, 16) * a.kv_heads;
+    uint32_t splits = most(1, 2048 / units);
+    splits = least(splits, least((tiles + 3) / 4, 128));
+    splits = slots > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / slots)));
+    p.chunk = (tiles + splits - 1) / splits;
+    p.splits = (tiles + p.chunk - 1) / p.chunk;
+    p.part_bytes = p.splits > 1 ? (size_t)slots * p.splits * 16 * (a.width + 4) * 4 : 0;
+    return p;
+}
+
 #ifdef __HIPCC__
 
 struct KvAppend {
@@ -110,7 +160,7 @@ struct PagedAttn {
     uint32_t* tickets;
     float* part;
 };
-hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, hipStream_t s);
+hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, const FewPlan& few, hipStream_t s);
 
 struct LogitsSelect {
     const float* logits;
@@ -133,10 +183,6 @@ struct LogitsSelect {
 hipError_t launch_logits_select(const LogitsSelect& a, hipStream_t s);
 
 #endif
-
-// A workspace starts with completion tickets, zero between calls; partial results follow.
-constexpr uint32_t kTickets = 16384;
-constexpr size_t kTicketBytes = kTickets * 4;
 
 // Tokens of a row's slice in the choice of a token, and the slices of a row.
 AF_HD uint32_t logits_slice(uint32_t rows, uint32_t vocabulary) {

@@ -225,11 +225,14 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const uint8_t* k_pages, co
 
 // ---- attention, key by key ----------------------------------------------------------------------------
 
-// Softmax attention of one query by one wave, key by key in fp32 over key tiles [t0, t1) of T keys: values are read
-// only where the query sees them.  Lane: channels E lane .. E lane + E - 1 (E = W / 64).
+// Softmax attention of one query by one wave, key by key in fp32 over key tiles t0, t0 + step, .. below t1 of T keys:
+// values are read only where the query sees them.  What the products below fall back to where a sum of theirs is
+// not finite: there an infinite cached value meets halves of a pair that are zero or of the other sign, also
+// of keys that the row does not see.  Lane: channels E lane .. E lane + E - 1 (E = W / 64).
 template <int W, bool Q4, uint32_t T>
-__device__ void plain_row(const PagedAttn& a, const Tiles& tiles, uint32_t t0, uint32_t t1, uint32_t seq, uint32_t h,
-                          int32_t pos, uint32_t end, const float (&q)[W / 64], float (&acc)[W / 64], float& m, float& l) {
+__device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles, uint32_t t0, uint32_t t1, uint32_t step,
+                                          uint32_t seq, uint32_t h, int32_t pos, uint32_t end, const float (&q)[W / 64],
+                                          float (&acc)[W / 64], float& m, float& l) {
     constexpr int E = W / 64;
     const uint32_t lane = threadIdx.x & 63, tokens = 1u << a.b.page_shift;
     const uint32_t bytes = page_part_bytes(Q4, tokens, W);
@@ -251,8 +254,10 @@ __device__ void plain_row(const PagedAttn& a, const Tiles& tiles, uint32_t t0, u
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
     m = -INFINITY;
     l = 0.0f;
-    for (uint32_t t = t0; t < t1; ++t) {
+#pragma unroll 1
+    for (uint32_t t = t0; t < t1; t += step) {
         const uint32_t j0 = tile_at(tiles, t) * T;
+#pragma unroll 1
         for (uint32_t j = j0; j < min(j0 + T, end); ++j) {
             if (!sees(pos, (int32_t)j, a.window, a.sinks)) continue;
             const uint32_t page = page_of(a.b, seq, (int32_t)j);
@@ -278,20 +283,495 @@ __device__ void plain_row(const PagedAttn& a, const Tiles& tiles, uint32_t t0, u
     }
 }
 
+// ---- attention of few rows: single tokens and short drafts ---------------------------------------------
+//
+// Rows are the (token, query head) pairs that share a KV head: row i of a sequence is token i / group, head i % group.
+// A block takes 16 of them against a chunk of the sequence's key tiles, its four waves tile by tile in turn; the
+// chunks of one row tile meet at a ticket, where the last block joins their partial sums (one pass over the
+// data with a running maximum and sum).  Bound by reading K and V once.
+//
+// Products are taken transposed on the fp16 matrix cores, S^T = K Q^T and O^T = V^T P^T (16 keys or channels by 16
+// rows): a lane holds one row's column throughout (row lane % 16), so the softmax needs two lane swaps per
+// tile and P is the second product's operand as it stands.  The order of the channels in the first sum and of the
+// keys in the second is free: lane group g = lane / 16 takes the channels its own 16-byte loads bring, and keys
+// 4 g .. 4 g + 3 of each half of a tile, so that K and V go from memory to operands in registers without LDS; V's
+// pairs of keys are made by byte permutes.  A half of a tile lies in one page (pages hold at least 16 tokens), so its
+// base address is scalar and every load adds a constant per lane.
+//
+// fp32 rows enter as fp16 pairs hi + lo (22 bits and more): queries scaled by a power of two to below 32,
+// probabilities times 2^14, which the exponent takes in.
+
+constexpr int kPartSC1 = 16;      // buffer access policy sc1: through to (or from) the memory side
+constexpr int kWaitVm0 = 0x0F70;  // s_waitcnt vmcnt(0), expcnt and lgkmcnt unconstrained
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kProbBits = 14.0f;
+
+// The first key that a query at position p sees, apart from the first tokens.
+__device__ __forceinline__ int32_t first_seen(int32_t p, uint32_t window) {
+    return window == 0 || window > 1u << 30 ? 0 : max(0, p + 1 - (int32_t)window);
+}
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float lanes4_max(float v) {
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const float w = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(w), __float_as_uint(w), false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
+__device__ __forceinline__ uint32_t pack2(_Float16 a, _Float16 b) { return __builtin_bit_cast(uint32_t, h2{a, b}); }
+
+// The step and lane group whose operand holds channels 8 o .. 8 o + 7 of a key's row.
 template <int W, bool Q4>
-__global__ __launch_bounds__(64) void paged_attention_plain_kernel(PagedAttn a, uint32_t q_heads) {
-    constexpr int E = W / 64;
-    const uint32_t token = blockIdx.x / q_heads, qh = blockIdx.x % q_heads, lane = threadIdx.x;
-    const uint32_t seq = sequence_of(a.b, token);
-    const Span s = span_of(a.b.starts[seq], a.b.starts[seq + 1], a.b.lengths[seq], a.b);
-    if (token < s.first || token - s.first >= s.count) return;
-    const int32_t pos = s.pos0 + (int32_t)(token - s.first);
-    const Tiles t = tiles_of<32>(pos, pos, s.end, a.window, a.sinks);
-    float q[E], acc[E], m, l;
-    for (int e = 0; e < E; ++e) q[e] = a.q[(size_t)token * a.q_stride + (size_t)qh * W + E * lane + e];
-    plain_row<W, Q4, 32>(a, t, 0, t.count, seq, qh / a.group, pos, s.end, q, acc, m, l);
-    float* o = a.out + (size_t)token * a.out_stride + (size_t)qh * W + E * lane;
-    for (int e = 0; e < E; ++e) o[e] = l == 0.0f ? 0.0f : acc[e] / l;
+__device__ __forceinline__ void operand_of(uint32_t o, uint32_t& step, uint32_t& g) {
+    if constexpr (!Q4) {
+        step = o / 4;
+        g = o % 4;
+    } else if constexpr (W >= 128) {  // a lane's 16-byte load of codes is one block of 32 channels: four steps
+        step = o / 16 * 4 + o % 4;
+        g = o / 4 % 4;
+    } else {
+        step = o % 2;
+        g = o / 2;
+    }
+}
+
+// Rows of K of one half tile (16 keys): a lane's loads, and its operand of a step.
+template <int W, bool Q4>
+struct KHalf {
+    v4u f[Q4 ? 1 : W / 32];
+    v4u c[Q4 ? (W >= 128 ? W / 128 : 1) : 1];
+    uint32_t d[Q4 ? (W >= 128 ? W / 128 : 1) : 1];  // (fp16 scales)
+
+    // part: the page's part, tokens: of a page, slot: of the half's first key
+    __device__ __forceinline__ void load(const uint8_t* part, uint32_t tokens, uint32_t slot, uint32_t lane) {
+        const uint32_t m = lane & 15, g = lane >> 4;
+        if constexpr (!Q4) {
+            const auto* p = gp(part + (size_t)slot * (W * 2)) + (m * (W * 2) + g * 16);
+#pragma unroll
+            for (int s = 0; s < W / 32; ++s) f[s] = *(const __attribute__((address_space(1))) v4u*)(p + 64 * s);
+        } else {
+            const auto* sc = gp(part + (size_t)tokens * (W / 2) + slot * (W / 16));
+            const auto* p = gp(part + (size_t)slot * (W / 2));
+            if constexpr (W >= 128) {
+#pragma unroll
+                for (int i = 0; i < W / 128; ++i) {
+                    c[i] = *(const __attribute__((address_space(1))) v4u*)(p + (m * (W / 2) + g * 16 + 64 * i));
+                    d[i] = *(const __attribute__((address_space(1))) uint16_t*)(sc + (m * (W / 16) + g * 2 + 8 * i));
+                }
+            } else {
+                const u2 w = *(const __attribute__((address_space(1))) u2*)(p + (m * (W / 2) + g * 8));
+                c[0] = v4u{w.x, w.y, 0u, 0u};
+                d[0] = *(const __attribute__((address_space(1))) uint16_t*)(sc + (m * (W / 16) + g / 2 * 2));
+            }
+        }
+    }
+    __device__ __forceinline__ h8 operand(int s) const {
+        if constexpr (!Q4) {
+            return __builtin_bit_cast(h8, f[s]);
+        } else {
+            h2 o[4];
+            unpack4(c[s / 4][s % 4], __builtin_bit_cast(_Float16, (uint16_t)d[s / 4]), o);
+            return h8{o[0].x, o[0].y, o[1].x, o[1].y, o[2].x, o[2].y, o[3].x, o[3].y};
+        }
+    }
+};
+
+// V of one half tile: a lane's four keys (4 g + j), channels 16 E (t / E) + E m + t % E of tile t in 0 .. W / 16 - 1.
+template <int W, bool Q4>
+struct VHalf {
+    static constexpr int E = Q4 ? W / 16 : (W / 16 < 8 ? W / 16 : 8);  // channels a load brings
+    static constexpr int C = W / 16 / E, R = Q4 ? (W / 128 ? W / 128 : 1) : E / 2;
+    uint32_t w[4][C][R];
+    uint32_t d[Q4 ? 4 : 1];  // (fp16 scales)
+
+    __device__ __forceinline__ void load(const uint8_t* part, uint32_t tokens, uint32_t slot, uint32_t lane) {
+        const uint32_t m = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (!Q4) {
+                const auto* p = gp(part + (size_t)slot * (W * 2)) + (g * (W * 8) + m * (2 * E) + j * (W * 2));
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    if constexpr (E == 8) {
+                        const v4u x = *(const __attribute__((address_space(1))) v4u*)(p + 256 * c);
+                        w[j][c][0] = x.x, w[j][c][1] = x.y, w[j][c][2] = x.z, w[j][c][3] = x.w;
+                    } else {
+                        const u2 x = *(const __attribute__((address_space(1))) u2*)(p);
+                        w[j][c][0] = x.x, w[j][c][1] = x.y;
+                    }
+            } else {
+                const auto* p = gp(part + (size_t)slot * (W / 2)) + (g * (W * 2) + m * (W / 32) + j * (W / 2));
+                if constexpr (W == 512) {
+                    const v4u x = *(const __attribute__((address_space(1))) v4u*)(p);
+                    w[j][0][0] = x.x, w[j][0][1] = x.y, w[j][0][2] = x.z, w[j][0][3] = x.w;
+                } else if constexpr (W == 256) {
+                    const u2 x = *(const __attribute__((address_space(1))) u2*)(p);
+                    w[j][0][0] = x.x, w[j][0][1] = x.y;
+                } else if constexpr (W == 128) {
+                    w[j][0][0] = *(const __attribute__((address_space(1))) uint32_t*)(p);
+                } else {  // four of a word's eight: pairs 0 and 1, or 2 and 3
+                    const auto* q = gp(part + (size_t)slot * (W / 2)) + (g * (W * 2) + m / 2 * 4 + j * (W / 2));
+                    w[j][0][0] = *(const __attribute__((address_space(1))) uint32_t*)(q) >> (m % 2 * 8);
+                }
+                d[j] = *(const __attribute__((address_space(1))) uint16_t*)(gp(part + (size_t)tokens * (W / 2) + slot * (W / 16)) +
+                                                                            (g * (W / 4) + m * W / 512 * 2 + j * (W / 16)));
+            }
+        }
+    }
+    // The lane's key j stands for zeros.
+    __device__ __forceinline__ void clear(int j) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int r = 0; r < R; ++r) w[j][c][r] = 0;
+        if constexpr (Q4) d[j] = 0;
+    }
+    // Operands of tiles 8 o .. (one octet of the lane's channels): per channel the halves' keys j, as pairs.
+    template <int N>
+    __device__ __forceinline__ void octet(int o, uint32_t (&k)[N][2]) const {
+        uint32_t x[4][N / 2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (!Q4) {
+#pragma unroll
+                for (int r = 0; r < N / 2; ++r) x[j][r] = w[j][o][r];
+            } else {
+                h2 p[4];
+                unpack4(w[j][0][o], __builtin_bit_cast(_Float16, (uint16_t)d[j]), p);
+#pragma unroll
+                for (int r = 0; r < N / 2; ++r) x[j][r] = __builtin_bit_cast(uint32_t, p[r]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                k[e][i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+    }
+};
+
+template <int W, bool Q4>
+__global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedAttn a, uint32_t units, uint32_t splits,
+                                                                          uint32_t row_tiles, uint32_t chunk) {
+    constexpr int ST = W / 32, TV = W / 16, HALFROWS = 8;
+    using V = VHalf<W, Q4>;
+    __shared__ __align__(16) uint8_t lds[W * 128];  // the queries' operands; at the end eight rows of each wave's sums
+    __shared__ float wm[4][16], wl[4][16];
+    __shared__ uint32_t last;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, g = lane >> 4;
+    const uint32_t split = blockIdx.x / units, unit = blockIdx.x % units;
+    const uint32_t h = unit % a.kv_heads, seq = unit / a.kv_heads % a.b.sequences, tile0 = unit / a.kv_heads / a.b.sequences;
+    const uint32_t start = a.b.starts[seq];
+    const Span s = span_of(start, a.b.starts[seq + 1], a.b.lengths[seq], a.b);
+    const uint32_t rows = s.count * a.group, tokens = 1u << a.b.page_shift;
+    const uint32_t part_bytes = page_part_bytes(Q4, tokens, W);
+    const uint32_t* table = a.b.table + (size_t)seq * a.b.table_stride;
+
+    // (one turn unless a sequence has more rows than the launch was told)
+    for (uint32_t rt = tile0; rt * 16 < rows; rt += row_tiles) {
+        const uint32_t nr = min(16u, rows - rt * 16);
+        const int32_t plo = s.pos0 + (int32_t)(rt * 16 / a.group), phi = s.pos0 + (int32_t)((rt * 16 + nr - 1) / a.group);
+        const Tiles keys = tiles_of<32>(plo, phi, s.end, a.window, a.sinks);
+        // the chunk of this block: at most `splits` of them
+        const uint32_t len = max(chunk, (keys.count + splits - 1) / splits);
+        const uint32_t parts = max(1u, (keys.count + len - 1) / len);
+        if (split >= parts) continue;
+        const uint32_t t0 = split * len + wave, t1 = min((split + 1) * len, keys.count);
+
+        // the pages of this wave's halves of tiles: lane l holds that of half l % 2 of its tile l / 2, 32 tiles at a time
+        uint32_t held = 0, held_at = t0;
+        auto pages_from = [&](uint32_t t) {
+            held_at = t;
+            const uint32_t i = t + lane / 2 * 4;
+            const uint32_t e = (tile_at(keys, min(i, max(keys.count, 1u) - 1)) * 32 + lane % 2 * 16) >> a.b.page_shift;
+            held = e < a.b.table_stride ? table[e] : a.b.pages;
+        };
+        KHalf<W, Q4> k[2];
+        V v[2];
+        bool ok[2] = {false, false};
+        auto bases = [&](uint32_t t, int half, size_t& off, uint32_t& slot) {
+            const uint32_t j = tile_at(keys, t) * 32 + half * 16;
+            uint32_t page = __builtin_amdgcn_readlane(held, (t - held_at) / 4 * 2 + half);
+            ok[half] = page < a.b.pages;
+            if (!ok[half]) page = 0;  // (some page: nothing of it is seen)
+            slot = j & (tokens - 1);
+            off = ((size_t)page * a.kv_heads + h) * part_bytes;
+        };
+        auto load_k = [&](uint32_t t) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                size_t off;
+                uint32_t slot;
+                bases(t, i, off, slot);
+                k[i].load(a.k_pages + off, tokens, slot, lane);
+            }
+        };
+        auto load_v = [&](uint32_t t) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                size_t off;
+                uint32_t slot;
+                bases(t, i, off, slot);
+                v[i].load(a.v_pages + off, tokens, slot, lane);
+            }
+        };
+        if (t0 < t1) {
+            pages_from(t0);
+            load_k(t0);
+            load_v(t0);
+        }
+
+        // the queries as scaled fp16 pairs in operand order: thread (row tid / 16, lane of 16) takes octets of channels
+        __syncthreads();  // (the last turn's sums are read)
+        float qs;         // of this lane's column: what a product has to be multiplied by
+        int32_t pos;
+        {
+            const uint32_t r = tid >> 4, c = tid & 15, row = rt * 16 + r;
+            constexpr int N = W >= 128 ? W / 128 : 1;
+            const bool on = r < nr && c < W / 8;
+            const float* src = a.q + (size_t)(s.first + row / a.group) * a.q_stride + (size_t)(h * a.group + row % a.group) * W;
+            float x[N][8], mx = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const f4 u = on ? *reinterpret_cast<const f4*>(src + 8 * (c + 16 * i)) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+                const f4 w = on ? *reinterpret_cast<const f4*>(src + 8 * (c + 16 * i) + 4) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[i][e] = u[e];
+                    x[i][4 + e] = w[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
+            }
+            const float up = query_scale(row_max(mx));
+            if (c < W / 8)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    h8 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float y = x[i][e] * up;
+                        hi[e] = (_Float16)y;
+                        lo[e] = (_Float16)(y - (float)hi[e]);
+                    }
+                    uint32_t step, og;
+                    operand_of<W, Q4>(c + 16 * i, step, og);
+                    *reinterpret_cast<h8*>(lds + ((step * 2 + 0) * 64 + og * 16 + r) * 16) = hi;
+                    *reinterpret_cast<h8*>(lds + ((step * 2 + 1) * 64 + og * 16 + r) * 16) = lo;
+                }
+            if (c == 0) wm[0][r] = a.scale / up * kLog2e;
+            __syncthreads();
+            qs = wm[0][m];
+            pos = s.pos0 + (int32_t)(min(rt * 16 + m, rows - 1) / a.group);  // (columns past the last row: as the last)
+        }
+        // a row at p sees keys [first_seen(p), p] and those below `first`; hi_m, lo_m: this lane's column, hi_all, lo_all:
+        // any row, hi_one, lo_one: every row
+        const int32_t edge = (int32_t)s.end - 1, first = (int32_t)min(a.sinks, 1u << 30);
+        const int32_t hi_m = min(pos, edge), hi_all = min(phi, edge), hi_one = min(plo, edge);
+        const int32_t lo_m = first_seen(pos, a.window), lo_all = first_seen(plo, a.window), lo_one = first_seen(phi, a.window);
+
+        f4 acc[TV];
+#pragma unroll
+        for (int t = 0; t < TV; ++t) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        float mrun = -INFINITY, lrun = 0.0f;  // (lrun: this lane's keys)
+#pragma unroll 1
+        for (uint32_t t = t0; t < t1; t += 4) {
+            const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
+            const bool ok0 = ok[0], ok1 = ok[1], more = t + 4 < t1;
+            f4 sv[2];
+            uint32_t qoff = lane * 16;
+            asm volatile("" : "+v"(qoff));  // (the queries stay in LDS: hoisted into registers they make the others spill)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;  // (the small products in a sum of their own)
+#pragma unroll
+                for (int st = 0; st < ST; ++st) {
+                    if (st % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                    const h8 A = k[i].operand(st);
+                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, *reinterpret_cast<const h8*>(lds + st * 2048 + qoff), x, 0, 0, 0);
+                    y = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, *reinterpret_cast<const h8*>(lds + st * 2048 + 1024 + qoff), y, 0, 0, 0);
+                }
+                sv[i] = (x + y) * qs;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) {
+                if (t + 4 >= held_at + 128) pages_from(t + 4);
+                load_k(t + 4);
+            }
+            // a whole tile: every row sees every key
+            const bool whole = ok0 & ok1 & (j0 + 31 <= hi_one) & ((j0 >= lo_one) | (j0 + 31 < first));
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int32_t j = j0 + 16 * i + 4 * (int32_t)g + e;
+                        const bool in = i ? ok1 : ok0;
+                        sv[i][e] = in & (j <= hi_m) & ((j >= lo_m) | (j < first)) ? sv[i][e] : -INFINITY;
+                        // keys that no row sees may be anything
+                        if (!(in & (j <= hi_all) & ((j >= lo_all) | (j < first)))) v[i].clear(e);
+                    }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
+                             fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
+            mx = fmaxf(mrun, lanes4_max(mx));
+            if (__ballot(mx > mrun)) {
+                const float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun - mx);
+                lrun *= al;
+#pragma unroll
+                for (int i = 0; i < TV; ++i) acc[i] *= al;
+                mrun = mx;
+            }
+            const float off = mrun == -INFINITY ? 0.0f : mrun - kProbBits;
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(sv[i][e] - off);
+                lrun += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const _Float16 a0 = (_Float16)p[2 * e], a1 = (_Float16)p[2 * e + 1];
+                    ph[2 * i + e] = pack2(a0, a1);
+                    pl[2 * i + e] = pack2((_Float16)(p[2 * e] - (float)a0), (_Float16)(p[2 * e + 1] - (float)a1));
+                }
+            }
+            const h8 bh = __builtin_bit_cast(h8, v4u{ph[0], ph[1], ph[2], ph[3]});
+            const h8 bl = __builtin_bit_cast(h8, v4u{pl[0], pl[1], pl[2], pl[3]});
+            constexpr int N = TV < 8 ? TV : 8;
+#pragma unroll
+            for (int o = 0; o < TV / N; ++o) {
+                __builtin_amdgcn_sched_barrier(0);
+                uint32_t x[N][2], y[N][2];
+                v[0].template octet<N>(o, x);
+                v[1].template octet<N>(o, y);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const h8 A = __builtin_bit_cast(h8, v4u{x[e][0], x[e][1], y[e][0], y[e][1]});
+                    acc[N * o + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[N * o + e], 0, 0, 0);
+                    acc[N * o + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[N * o + e], 0, 0, 0);
+                }
+            }
+            if (more) load_v(t + 4);
+        }
+        lrun = row_total(lrun);
+
+        // columns whose sums are not finite
+        float zero = lrun * 0.0f;
+#pragma unroll
+        for (int t = 0; t < TV; ++t) zero += (acc[t][0] + acc[t][1] + acc[t][2] + acc[t][3]) * 0.0f;
+        uint64_t odd = __ballot(!(zero == 0.0f));
+        odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;
+
+        // the waves' sums meet in LDS, eight rows at a time
+        float* sums = reinterpret_cast<float*>(lds);  // [wave][row of 8][W]
+        const uint32_t slot = (start * a.group / 16 + seq + rt) * a.kv_heads + h;
+        float* part = a.part + ((size_t)slot * splits + split) * 16 * (W + 4);
+        __syncthreads();  // every wave is past its queries
+        if (lane < 16) {
+            wm[wave][m] = mrun;
+            wl[wave][m] = lrun;
+        }
+#pragma unroll 1
+        for (uint32_t r0 = 0; r0 < nr; r0 += HALFROWS) {
+            if (r0) __syncthreads();
+            const uint32_t r = m - r0;
+            if (r < HALFROWS && m < nr) {
+                float* dst = sums + (wave * HALFROWS + r) * W;
+#pragma unroll
+                for (int t = 0; t < TV; t += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<f4*>(dst + 16 * V::E * (t / V::E) + V::E * (4 * g + e) + t % V::E) =
+                            f4{acc[t][e], acc[t + 1][e], acc[t + 2][e], acc[t + 3][e]};
+            }
+            for (uint32_t bad = (uint32_t)(odd >> r0) & 0xFF; bad; bad &= bad - 1) {
+                const uint32_t c = r0 + __builtin_ctz(bad);
+                if (c >= nr) break;
+                const uint32_t row = rt * 16 + c;
+                constexpr int E = W / 64;
+                float q[E], o[E], pm, pl2;
+                const float* src = a.q + (size_t)(s.first + row / a.group) * a.q_stride + (size_t)(h * a.group + row % a.group) * W;
+#pragma unroll
+                for (int e = 0; e < E; ++e) q[e] = src[E * lane + e];
+                plain_row<W, Q4, 32>(a, keys, t0, t1, 4, seq, h, s.pos0 + (int32_t)(row / a.group), s.end, q, o, pm, pl2);
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int e = 0; e < E; ++e) sums[(wave * HALFROWS + c - r0) * W + E * lane + e] = o[e];
+                if (lane == 0) {
+                    wm[wave][c] = pm * kLog2e + kProbBits;  // (its sums lack the others' 2^14)
+                    wl[wave][c] = pl2;
+                }
+            }
+            __syncthreads();
+            for (uint32_t i = tid; i < min((uint32_t)HALFROWS, nr - r0) * (W / 4); i += 256) {
+                const uint32_t c = i / (W / 4), x = i % (W / 4) * 4, row = rt * 16 + r0 + c;
+                float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) M = fmaxf(M, wm[w][r0 + c]);
+                f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float f = wm[w][r0 + c] == -INFINITY && wl[w][r0 + c] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(wm[w][r0 + c] - M);
+                    L = fmaf(f, wl[w][r0 + c], L);
+                    if (f != 0.0f) o += f * *reinterpret_cast<const f4*>(sums + (w * HALFROWS + c) * W + x);
+                }
+                if (parts == 1) {
+                    float* out = a.out + (size_t)(s.first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;
+                    *reinterpret_cast<f4*>(out + x) = L == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o / L;
+                } else {
+                    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(part, 0, 16 * (W + 4) * 4, 0x00020000);
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, o), rs, ((r0 + c) * (W + 4) + x) * 4, 0, kPartSC1);
+                    if (x == 0)
+                        __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(M), __float_as_uint(L)}, rs,
+                                                              ((r0 + c) * (W + 4) + W) * 4, 0, kPartSC1);
+                }
+            }
+        }
+        if (parts == 1) continue;
+        // the chunks meet at the slot's ticket; the last block joins them in order
+        __builtin_amdgcn_s_waitcnt(kWaitVm0);
+        __syncthreads();
+        if (tid == 0)
+            last = __hip_atomic_fetch_add(a.tickets + slot, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+        __syncthreads();
+        if (!last) continue;
+        if (tid == 0) __hip_atomic_store(a.tickets + slot, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            a.part + (size_t)slot * splits * 16 * (W + 4), 0, (int)(splits * 16 * (W + 4) * 4), 0x00020000);
+        for (uint32_t i = tid; i < nr * (W / 4); i += 256) {
+            const uint32_t c = i / (W / 4), x = i % (W / 4) * 4, row = rt * 16 + c;
+            float M = -INFINITY, L = 0.0f;
+            f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t p0 = 0; p0 < parts; p0 += 8) {
+                u2 ml[8];
+                v4u sv[8];
+#pragma unroll
+                for (uint32_t u = 0; u < 8; ++u) {
+                    const uint32_t at = (min(p0 + u, parts - 1) * 16 + c) * (W + 4);
+                    ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, (at + W) * 4, 0, kPartSC1);
+                    sv[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (at + x) * 4, 0, kPartSC1);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < 8; ++u) {
+                    const float pm = __uint_as_float(ml[u].x), pl = __uint_as_float(ml[u].y);
+                    if (p0 + u >= parts || (pm == -INFINITY && pl == 0.0f)) continue;
+                    const float mn = fmaxf(M, pm);
+                    const float al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(pm - mn);
+                    L = L * al + pl * f;
+                    o = (al == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o * al) + (f == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : __builtin_bit_cast(f4, sv[u]) * f);
+                    M = mn;
+                }
+            }
+            float* out = a.out + (size_t)(s.first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;
+            *reinterpret_cast<f4*>(out + x) = L == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o / L;
+        }
+    }
 }
 
 }  // namespace
@@ -329,11 +809,11 @@ hipError_t launch_kv_read(const uint8_t* k_pages, const uint8_t* v_pages, const 
     });
 }
 
-hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, hipStream_t s) {
-    const uint32_t q_heads = a.kv_heads * a.group;
+hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, const FewPlan& few, hipStream_t s) {
+    const uint32_t units = few.row_tiles * a.b.sequences * a.kv_heads;
     return by_layout(width, q4, [&](auto w, auto t) {
-        hipLaunchKernelGGL((paged_attention_plain_kernel<decltype(w)::value, decltype(t)::value>), dim3(a.b.tokens * q_heads),
-                           dim3(64), 0, s, a, q_heads);
+        hipLaunchKernelGGL((paged_few_kernel<decltype(w)::value, decltype(t)::value>), dim3(units * few.splits), dim3(256), 0, s,
+                           a, units, few.splits, few.row_tiles, few.chunk);
         return hipGetLastError();
     });
 }

@@ -3,6 +3,7 @@
 // free functions, so all of them can be captured into graphs.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -38,10 +39,14 @@ int current_device(int* out) {
     if (hipGetDeviceCount(&n) != hipSuccess || n < 1) return fail(AF_ERR_NO_DEVICE, "no HIP device");
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return fail(e, "current device");
-    hipDeviceProp_t p;
-    if ((e = hipGetDeviceProperties(&p, dev)) != hipSuccess) return fail(e, "device properties");
-    if (std::strncmp(p.gcnArchName, "gfx950", 6) != 0)
-        return set_error(AF_ERR_NO_DEVICE, std::string("gfx950 (MI355X) required, found ") + p.gcnArchName);
+    static std::atomic<uint64_t> known{0};  // devices already seen to be gfx950 (asking takes about 0.1 ms)
+    if (dev >= 64 || !(known.load() >> dev & 1)) {
+        hipDeviceProp_t p;
+        if ((e = hipGetDeviceProperties(&p, dev)) != hipSuccess) return fail(e, "device properties");
+        if (std::strncmp(p.gcnArchName, "gfx950", 6) != 0)
+            return set_error(AF_ERR_NO_DEVICE, std::string("gfx950 (MI355X) required, found ") + p.gcnArchName);
+        if (dev < 64) known.fetch_or(1ull << dev);
+    }
     *out = dev;
     return AF_OK;
 }
@@ -111,7 +116,14 @@ int check_attention_sizes(const af_paged_attention_args& a) {
         return fail(AF_ERR_INVALID, "unsupported cache layout (type, 16 to 256 tokens a page, 1 to 1024 heads, width 64, 128, 256 or 512)");
     if (a.batch.sequences == 0 || a.batch.sequences > AF_MAX_SEQUENCES || a.batch.tokens == 0 || a.batch.tokens > AF_MAX_BATCH_TOKENS)
         return fail(AF_ERR_INVALID, "invalid number of sequences or batch tokens");
+    if ((uint64_t)a.batch.sequences * c.kv_heads > 1u << 22) return fail(AF_ERR_INVALID, "sequences times KV heads above 4194304");
     return AF_OK;
+}
+
+AttnShape shape_of(const af_paged_attention_args& a) {
+    const af_attention_config& c = a.config;
+    return {a.batch.sequences, a.batch.tokens,    c.kv_heads,        c.q_heads / c.kv_heads, c.width, c.window, a.sinks,
+            a.longest_query,   a.longest_context, least(a.batch.table_stride, AF_MAX_POSITIONS / a.pages.page) * a.pages.page};
 }
 
 }  // namespace
@@ -257,7 +269,7 @@ int af_paged_attention_workspace(const af_paged_attention_args* p, size_t* bytes
     if (!p || !bytes) return fail(AF_ERR_INVALID, "null argument");
     const int rc = check_attention_sizes(*p);
     if (rc) return rc;
-    *bytes = kTicketBytes;
+    *bytes = kTicketBytes + few_plan(shape_of(*p)).part_bytes;
     return AF_OK;
 }
 
@@ -287,7 +299,7 @@ int af_paged_attention(const af_paged_attention_args* p, void* stream) {
     a.b = batch_view(p->batch, p->pages);
     a.tickets = (uint32_t*)p->workspace->p;
     a.part = (float*)((char*)p->workspace->p + kTicketBytes);
-    const hipError_t e = launch_paged_attention(a, p->config.width, p->pages.type == AF_KV_Q4, (hipStream_t)stream);
+    const hipError_t e = launch_paged_attention(a, p->config.width, p->pages.type == AF_KV_Q4, few_plan(shape_of(*p)), (hipStream_t)stream);
     return e == hipSuccess ? AF_OK : fail(e, "paged attention launch");
 }
 
