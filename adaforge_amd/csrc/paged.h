@@ -106,26 +106,41 @@ AF_HD uint32_t longest_tiles(const AttnShape& a, uint32_t tokens) {
     return (keys + 31) / 32;
 }
 
-// The launch over few rows: grid units (row tiles of 16, sequences, KV heads) by splits, each split a chunk of key tiles.
-struct FewPlan {
-    uint32_t row_tiles, splits, chunk;
+// A launch: row tiles of `rows` rows, their keys in at most `splits` chunks of `chunk` tiles or more.  16 rows: grid
+// units (row tiles, sequences, KV heads) by splits; more: grid slots, KV heads and splits.
+struct AttnPlan {
+    uint32_t rows, units, row_tiles, slots, splits, chunk;
+    bool join_apart;  // the chunks are joined by a launch of their own
     size_t part_bytes;
 };
 
-AF_HD FewPlan few_plan(const AttnShape& a) {
-    FewPlan p;
+AF_HD AttnPlan attn_plan(const AttnShape& a) {
+    AttnPlan p;
     const uint32_t tokens = most(1, least(a.longest_query, a.tokens));
     const uint64_t pairs = (uint64_t)a.sequences * a.kv_heads;  // (at most 2^22: checked by the call)
+    const uint32_t tiles = longest_tiles(a, tokens);
     p.row_tiles = (uint32_t)(((uint64_t)tokens * a.group + 15) / 16);
+    p.rows = p.row_tiles > 1 ? (a.width == 512 || (uint64_t)row_slots(a, 128) * a.kv_heads < 256 ? 64 : 128) : 16;
+    p.slots = row_slots(a, p.rows);
     if (p.row_tiles * pairs > 1u << 22) p.row_tiles = most(1, (uint32_t)((1u << 22) / pairs));
-    const uint32_t units = (uint32_t)(p.row_tiles * pairs), tiles = longest_tiles(a, tokens);
-    const uint64_t slots = (uint64_t)row_slots(a, 16) * a.kv_heads;
-    uint32_t splits = most(1, 2048 / units);
-    splits = least(splits, least((tiles + 3) / 4, 128));
-    splits = slots > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / slots)));
+    const uint64_t sums = (uint64_t)p.slots * a.kv_heads;
+    uint32_t splits;
+    if (p.rows == 16) {
+        p.units = (uint32_t)(p.row_tiles * pairs);
+        // as many chunks as fill the chip, then more of at least 32 tiles for lengths that differ
+        const uint32_t fill = least(most(1, 256 / p.units), (tiles + 3) / 4), even = least(most(1, 2048 / p.units), most(1, tiles / 32));
+        splits = least(most(fill, even), 128);
+        splits = sums > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / sums)));
+    } else {
+        p.units = (uint32_t)sums;
+        splits = least(most(1, 1024 / p.units), most(1, tiles / 16));
+        splits = least(splits, 16);
+    }
     p.chunk = (tiles + splits - 1) / splits;
     p.splits = (tiles + p.chunk - 1) / p.chunk;
-    p.part_bytes = p.splits > 1 ? (size_t)slots * p.splits * 16 * (a.width + 4) * 4 : 0;
+    const uint64_t row_bytes = (uint64_t)(a.width + 4) * 4;
+    p.join_apart = p.splits > 1 && (p.rows > 16 || p.splits * least(16, tokens * a.group) * row_bytes > 65536);
+    p.part_bytes = p.splits > 1 ? (size_t)(sums * p.splits * p.rows * row_bytes) : 0;
     return p;
 }
 
@@ -160,7 +175,7 @@ struct PagedAttn {
     uint32_t* tickets;
     float* part;
 };
-hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, const FewPlan& few, hipStream_t s);
+hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, const AttnPlan& plan, hipStream_t s);
 
 struct LogitsSelect {
     const float* logits;

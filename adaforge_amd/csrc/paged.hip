@@ -9,20 +9,26 @@ namespace {
 
 // ---- where a batch's rows stand ------------------------------------------------------------------
 
-// The sequence whose rows hold row `token` (wave-uniform; the last s with starts[s] <= token), searched 64 ways at a
-// time: one round of loads for up to 64 sequences.
-__device__ __forceinline__ uint32_t sequence_of(const PagedBatch& b, uint32_t token) {
-    uint32_t lo = 0, n = b.sequences;
+// The last sequence s with before(s) true (wave-uniform; 0 if there is none), for before that holds up to some s:
+// searched 64 ways at a time, one round of loads for up to 64 sequences.
+template <typename F>
+__device__ __forceinline__ uint32_t last_sequence(uint32_t sequences, F before) {
+    uint32_t lo = 0, n = sequences;
     const uint32_t lane = threadIdx.x & 63;
     while (n > 1) {
         const uint32_t step = (n + 63) / 64, i = lane * step;
-        const bool at = i < n && b.starts[lo + i] <= token;
+        const bool at = i < n && before(lo + i);
         const uint32_t k = __popcll(__ballot(at));
         const uint32_t skip = k ? (k - 1) * step : 0;
         lo += skip;
         n = min(step, n - skip);
     }
     return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// The sequence whose rows hold row `token`.
+__device__ __forceinline__ uint32_t sequence_of(const PagedBatch& b, uint32_t token) {
+    return last_sequence(b.sequences, [&](uint32_t s) { return b.starts[s] <= token; });
 }
 
 struct Place {
@@ -454,9 +460,56 @@ struct VHalf {
     }
 };
 
+// The chunks of a row tile of `tiles` key tiles: chunk tiles each, or more where they would be over `splits`.
+__device__ __forceinline__ void chunks_of(uint32_t tiles, uint32_t chunk, uint32_t splits, uint32_t& len, uint32_t& parts) {
+    len = max(chunk, (tiles + splits - 1) / splits);
+    parts = max(1u, (tiles + len - 1) / len);
+}
+
+// Adds sums (o, L) of maximum m to those of maximum M, as weights 2^m; a chunk that saw nothing has m = -inf, l = 0.
+__device__ __forceinline__ void join(f4& o, float& L, float& M, const f4& v, float l, float m) {
+    if (m == -INFINITY && l == 0.0f) return;
+    const float mn = fmaxf(M, m);
+    const float al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(m - mn);
+    const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};  // (no infinity times a zero weight)
+    L = L * al + l * f;
+    o = (al == 0.0f ? zero : o * al) + (f == 0.0f ? zero : v * f);
+    M = mn;
+}
+
+// Rows [c0, nr) of a row tile from its chunks' partial sums, [parts][R][W + 4], every nth quad of channels by a thread.
+template <int W>
+__device__ __forceinline__ void join_parts(const PagedAttn& a, const float* part, uint32_t splits, uint32_t parts, uint32_t R,
+                                           uint32_t c0, uint32_t nr, uint32_t row0, uint32_t first, uint32_t h) {
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, (int)(splits * R * (W + 4) * 4), 0x00020000);
+    for (uint32_t i = threadIdx.x; i < (nr - c0) * (W / 4); i += 256) {
+        const uint32_t c = c0 + i / (W / 4), x = i % (W / 4) * 4, row = row0 + c;
+        float M = -INFINITY, L = 0.0f;
+        f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t p0 = 0; p0 < parts; p0 += 8) {
+            u2 ml[8];
+            v4u sv[8];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) {
+                const uint32_t at = (min(p0 + u, parts - 1) * R + c) * (W + 4);
+                ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, (at + W) * 4, 0, kPartSC1);
+                sv[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (at + x) * 4, 0, kPartSC1);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u)
+                if (p0 + u < parts)
+                    join(o, L, M, __builtin_bit_cast(f4, sv[u]), __uint_as_float(ml[u].y), __uint_as_float(ml[u].x));
+        }
+        float* out = a.out + (size_t)(first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;
+        *reinterpret_cast<f4*>(out + x) = L == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o / L;
+    }
+}
+
+// join_apart: the chunks are joined by paged_join_kernel afterwards, not by the last of them.
 template <int W, bool Q4>
 __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedAttn a, uint32_t units, uint32_t splits,
-                                                                          uint32_t row_tiles, uint32_t chunk) {
+                                                                          uint32_t row_tiles, uint32_t chunk, bool join_apart) {
     constexpr int ST = W / 32, TV = W / 16, HALFROWS = 8;
     using V = VHalf<W, Q4>;
     __shared__ __align__(16) uint8_t lds[W * 128];  // the queries' operands; at the end eight rows of each wave's sums
@@ -477,8 +530,8 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         const int32_t plo = s.pos0 + (int32_t)(rt * 16 / a.group), phi = s.pos0 + (int32_t)((rt * 16 + nr - 1) / a.group);
         const Tiles keys = tiles_of<32>(plo, phi, s.end, a.window, a.sinks);
         // the chunk of this block: at most `splits` of them
-        const uint32_t len = max(chunk, (keys.count + splits - 1) / splits);
-        const uint32_t parts = max(1u, (keys.count + len - 1) / len);
+        uint32_t len, parts;
+        chunks_of(keys.count, chunk, splits, len, parts);
         if (split >= parts) continue;
         const uint32_t t0 = split * len + wave, t1 = min((split + 1) * len, keys.count);
 
@@ -733,7 +786,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                 }
             }
         }
-        if (parts == 1) continue;
+        if (parts == 1 || join_apart) continue;
         // the chunks meet at the slot's ticket; the last block joins them in order
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
         __syncthreads();
@@ -742,34 +795,392 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         __syncthreads();
         if (!last) continue;
         if (tid == 0) __hip_atomic_store(a.tickets + slot, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            a.part + (size_t)slot * splits * 16 * (W + 4), 0, (int)(splits * 16 * (W + 4) * 4), 0x00020000);
-        for (uint32_t i = tid; i < nr * (W / 4); i += 256) {
-            const uint32_t c = i / (W / 4), x = i % (W / 4) * 4, row = rt * 16 + c;
-            float M = -INFINITY, L = 0.0f;
-            f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t p0 = 0; p0 < parts; p0 += 8) {
-                u2 ml[8];
-                v4u sv[8];
+        join_parts<W>(a, a.part + (size_t)slot * splits * 16 * (W + 4), splits, parts, 16, 0, nr, rt * 16, s.first, h);
+    }
+}
+
+// The sequence and row tile (of R rows) of a partial-sum slot.
+__device__ __forceinline__ uint32_t slot_sequence(const PagedAttn& a, uint32_t slot, uint32_t R, uint32_t& tile) {
+    const PagedBatch& b = a.b;
+    auto base = [&](uint32_t s) { return (uint32_t)((uint64_t)min(b.starts[s], b.tokens) * a.group / R) + s; };
+    const uint32_t seq = last_sequence(b.sequences, [&](uint32_t s) { return base(s) <= slot; });
+    tile = slot - min(slot, base(seq));
+    return seq;
+}
+
+// Joins the chunks of (row tile, KV head) slots: a block per 1,024 sums of a slot, so that wide tiles of many chunks
+// are read by many CUs.
+template <int W>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t splits, uint32_t chunk, uint32_t R) {
+    constexpr uint32_t C = 1024 / W < 1 ? 1 : 1024 / W;  // rows of a block
+    const uint32_t groups = R / C, slot = blockIdx.x / groups, c0 = blockIdx.x % groups * C, h = slot % a.kv_heads;
+    uint32_t tile;
+    const uint32_t seq = slot_sequence(a, slot / a.kv_heads, R, tile);
+    const Span s = span_of(a.b.starts[seq], a.b.starts[seq + 1], a.b.lengths[seq], a.b);
+    const uint32_t rows = s.count * a.group;
+    if (tile * R >= rows) return;
+    const uint32_t nr = min(R, rows - tile * R);
+    if (c0 >= nr) return;
+    const int32_t plo = s.pos0 + (int32_t)(tile * R / a.group), phi = s.pos0 + (int32_t)((tile * R + nr - 1) / a.group);
+    const Tiles keys = tiles_of<32>(plo, phi, s.end, a.window, a.sinks);
+    uint32_t len, parts;
+    chunks_of(keys.count, chunk, splits, len, parts);
+    if (parts == 1) return;
+    join_parts<W>(a, a.part + (size_t)slot * splits * R * (W + 4), splits, parts, R, c0, min(nr, c0 + C), tile * R, s.first, h);
+}
+
+// ---- attention of many rows: prompts and further turns --------------------------------------------------
+//
+// Row tiles of 64 NQ rows: a wave holds 16 NQ of them from scores to output, their queries and sums in registers, and
+// the block's four waves share K and V through LDS, 32 keys at a time in two buffers: while one tile is used, the next
+// one is on its way (in registers, then in the other buffer) and one barrier separates tiles.  Bound by the matrix
+// cores' 8 W multiply-adds per (row, key): both operands' pairs double the 4 W of the product.
+//
+// K lies in LDS as the first product reads it, piece ((half, step), lane) of 16 bytes; V transposed and its channels
+// ordered by their place in an octet (E values of a load), so that writes (lanes along octets and keys) and reads
+// (lanes along a tile's 16 rows) both sweep LDS in address order.  Q4 blocks become fp16 on the way.
+
+template <int W, bool Q4, int NQ>
+__global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(PagedAttn a, uint32_t slots, uint32_t splits,
+                                                                                uint32_t chunk) {
+    constexpr int ST = W / 32, TV = W / 16, R = 64 * NQ;
+    constexpr int E = W / 16 < 8 ? W / 16 : 8;  // channels of an octet
+    constexpr int NK = Q4 ? (W + 255) / 256 : W / 64;  // a thread's pieces of K: blocks of 32 values, or octets
+    constexpr int NV = (W + 255) / 256;                // and of V: four keys of an octet of channels
+    __shared__ __align__(16) uint8_t lds[2][2][W * 64];  // [buffer][K, V]
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, g = lane >> 4;
+    // blocks b and b + 8 share an XCD: with heads times splits a multiple of 8, a head's row tiles share an L2
+    const uint32_t heads = a.kv_heads * splits;
+    uint32_t hs, slot;
+    if (heads % 8 == 0) {
+        hs = blockIdx.x / 8 / slots * 8 + blockIdx.x % 8;
+        slot = blockIdx.x / 8 % slots;
+    } else {
+        hs = blockIdx.x / slots;
+        slot = blockIdx.x % slots;
+    }
+    slot = slots - 1 - slot;  // (a sequence's last rows, which see the most keys, first)
+    const uint32_t h = hs % a.kv_heads, split = hs / a.kv_heads;
+    uint32_t rt;
+    const uint32_t seq = slot_sequence(a, slot, R, rt);
+    const Span s = span_of(a.b.starts[seq], a.b.starts[seq + 1], a.b.lengths[seq], a.b);
+    const uint32_t rows = s.count * a.group, tokens = 1u << a.b.page_shift;
+    if (rt * R >= rows) return;
+    const uint32_t nr = min((uint32_t)R, rows - rt * R);
+    const int32_t plo = s.pos0 + (int32_t)(rt * R / a.group), phi = s.pos0 + (int32_t)((rt * R + nr - 1) / a.group);
+    const Tiles keys = tiles_of<32>(plo, phi, s.end, a.window, a.sinks);
+    uint32_t len, parts;
+    chunks_of(keys.count, chunk, splits, len, parts);
+    if (split >= parts) return;
+    const uint32_t t0 = split * len, t1 = min(t0 + len, keys.count);
+    const uint32_t part_bytes = page_part_bytes(Q4, tokens, W);
+    const uint32_t* table = a.b.table + (size_t)seq * a.b.table_stride;
+    const int32_t edge = (int32_t)s.end - 1, first = (int32_t)min(a.sinks, 1u << 30);
+    const int32_t hi_all = min(phi, edge), lo_all = first_seen(plo, a.window);
+
+    // page numbers: lane l holds that of half l % 2 of tile held_at + l / 2
+    uint32_t held = 0, held_at = t0;
+    auto pages_from = [&](uint32_t t) {
+        held_at = t;
+        const uint32_t e = (tile_at(keys, min(t + lane / 2, keys.count - 1)) * 32 + lane % 2 * 16) >> a.b.page_shift;
+        held = e < a.b.table_stride ? table[e] : a.b.pages;
+    };
+    // the next tile's K and V on their way
+    v4u kr[NK];
+    uint32_t kd[Q4 ? NK : 1];
+    uint32_t vr[NV][4][Q4 ? 1 : 4], vd[Q4 ? NV : 1][4];
+    auto load = [&](uint32_t t) {
+        if (t >= held_at + 32) pages_from(t);
+        const uint32_t j0 = tile_at(keys, t) * 32;
+        size_t off[2];
+        uint32_t slot_[2];
 #pragma unroll
-                for (uint32_t u = 0; u < 8; ++u) {
-                    const uint32_t at = (min(p0 + u, parts - 1) * 16 + c) * (W + 4);
-                    ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, (at + W) * 4, 0, kPartSC1);
-                    sv[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (at + x) * 4, 0, kPartSC1);
+        for (int i = 0; i < 2; ++i) {
+            uint32_t page = __builtin_amdgcn_readlane(held, (t - held_at) * 2 + i);
+            if (page >= a.b.pages) page = 0;  // (some page: nothing of it is seen)
+            slot_[i] = (j0 + 16 * i) & (tokens - 1);
+            off[i] = ((size_t)page * a.kv_heads + h) * part_bytes;
+        }
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const uint32_t e = tid + 256 * i;
+            if constexpr (!Q4) {  // octet e: half, step, group, row
+                const uint32_t half = e / 64 / ST, st = e / 64 % ST;
+                const uint8_t* p = a.k_pages + (half ? off[1] : off[0]) + ((half ? slot_[1] : slot_[0]) + e % 16) * (W * 2) + st * 64 + e / 16 % 4 * 16;
+                kr[i] = *gp(reinterpret_cast<const v4u*>(p));
+            } else if (W >= 256 || e < W) {  // block e: half, block, row
+                const uint32_t half = e / 16 / ST, b = e / 16 % ST, sl = (half ? slot_[1] : slot_[0]) + e % 16;
+                const uint8_t* p = a.k_pages + (half ? off[1] : off[0]);
+                kr[i] = *gp(reinterpret_cast<const v4u*>(p + sl * (W / 2) + b * 16));
+                kd[i] = *gp(reinterpret_cast<const uint16_t*>(p + tokens * (W / 2) + sl * (W / 16) + b * 2));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t e = tid + 256 * i, u = e % 8, o = e / 8;  // keys 16 (u / 4) + 4 (u % 4) .. + 3, octet o of 8 channels
+            if (W < 256 && e >= W) break;
+            const uint8_t* p = a.v_pages + (u / 4 ? off[1] : off[0]);
+            const uint32_t sl = (u / 4 ? slot_[1] : slot_[0]) + u % 4 * 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if constexpr (!Q4) {
+                    const v4u x = *gp(reinterpret_cast<const v4u*>(p + (sl + j) * (W * 2) + o * 16));
+                    vr[i][j][0] = x.x, vr[i][j][1] = x.y, vr[i][j][2] = x.z, vr[i][j][3] = x.w;
+                } else {
+                    vr[i][j][0] = *gp(reinterpret_cast<const uint32_t*>(p + (sl + j) * (W / 2) + o * 4));
+                    vd[i][j] = *gp(reinterpret_cast<const uint16_t*>(p + tokens * (W / 2) + (sl + j) * (W / 16) + o / 4 * 2));
                 }
+        }
+    };
+    auto store = [&](uint32_t t, uint8_t* kl, uint8_t* vl) {
+        const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
 #pragma unroll
-                for (uint32_t u = 0; u < 8; ++u) {
-                    const float pm = __uint_as_float(ml[u].x), pl = __uint_as_float(ml[u].y);
-                    if (p0 + u >= parts || (pm == -INFINITY && pl == 0.0f)) continue;
-                    const float mn = fmaxf(M, pm);
-                    const float al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(pm - mn);
-                    L = L * al + pl * f;
-                    o = (al == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o * al) + (f == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : __builtin_bit_cast(f4, sv[u]) * f);
-                    M = mn;
+        for (int i = 0; i < NK; ++i) {
+            const uint32_t e = tid + 256 * i;
+            if constexpr (!Q4) {
+                *reinterpret_cast<v4u*>(kl + e * 16) = kr[i];
+            } else if (W >= 256 || e < W) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    h2 x[4];
+                    unpack4(kr[i][w], __builtin_bit_cast(_Float16, (uint16_t)kd[i]), x);
+                    *reinterpret_cast<v4u*>(kl + (e / 16 * 64 + w * 16 + e % 16) * 16) =
+                        v4u{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1]),
+                            __builtin_bit_cast(uint32_t, x[2]), __builtin_bit_cast(uint32_t, x[3])};
                 }
             }
+        }
+        const bool p0 = __builtin_amdgcn_readlane(held, (t - held_at) * 2) < a.b.pages;
+        const bool p1 = __builtin_amdgcn_readlane(held, (t - held_at) * 2 + 1) < a.b.pages;
+        const bool whole = p0 & p1 & (j0 + 31 <= hi_all) & ((j0 >= lo_all) | (j0 + 31 < first));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t e = tid + 256 * i, u = e % 8, o = e / 8;
+            if (W < 256 && e >= W) break;
+            uint32_t x[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (!Q4) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[j][r] = vr[i][j][r];
+                } else {
+                    h2 y[4];
+                    unpack4(vr[i][j][0], __builtin_bit_cast(_Float16, (uint16_t)vd[i][j]), y);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[j][r] = __builtin_bit_cast(uint32_t, y[r]);
+                }
+            }
+            if (!whole)  // keys that no row sees may be anything
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int32_t key = j0 + (int32_t)(u * 4) + j;
+                    if (!((u / 4 ? p1 : p0) & (key <= hi_all) & ((key >= lo_all) | (key < first))))
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[j][r] = 0;
+                }
+            // channel c: row (c % E) W / E + c / E of the transposed tile; piece u % 4 of 8 keys, its half u / 4
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
+                const uint32_t at = (d % E) * (W / E) + o * (8 / E) + d / E;
+                *reinterpret_cast<u2*>(vl + at * 64 + u % 4 * 16 + u / 4 * 8) =
+                    u2{__builtin_amdgcn_perm(x[1][d / 2], x[0][d / 2], sel), __builtin_amdgcn_perm(x[3][d / 2], x[2][d / 2], sel)};
+            }
+        }
+    };
+    if (t0 < t1) {
+        pages_from(t0);
+        load(t0);
+    }
+
+    // the queries: lane (column m, g) holds channels 32 s + 8 g .. + 7 of step s, as scaled fp16 pairs
+    h8 qh[NQ][ST], ql[NQ][ST];
+    float qs[NQ];
+    int32_t pos[NQ];
+    const uint32_t row0 = rt * R + wave * (16 * NQ);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const uint32_t row = min(row0 + 16 * n + m, rows - 1);  // (columns past the last row: as the last)
+        const float* src = a.q + (size_t)(s.first + row / a.group) * a.q_stride + (size_t)(h * a.group + row % a.group) * W + 8 * g;
+        pos[n] = s.pos0 + (int32_t)(row / a.group);
+        float mx = 0.0f;
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const f4 x = *gp(reinterpret_cast<const f4*>(src + 32 * st + 4 * i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[e]));
+            }
+        const float up = query_scale(lanes4_max(mx));
+        qs[n] = a.scale / up * kLog2e;
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const f4 x = *gp(reinterpret_cast<const f4*>(src + 32 * st + 4 * i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = x[e] * up;
+                    qh[n][st][4 * i + e] = (_Float16)y;
+                    ql[n][st][4 * i + e] = (_Float16)(y - (float)qh[n][st][4 * i + e]);
+                }
+            }
+    }
+    // this wave's rows: what any and what every one of them sees
+    const bool idle = row0 >= rows;
+    const int32_t wlo = s.pos0 + (int32_t)(min(row0, rows - 1) / a.group);
+    const int32_t whi = s.pos0 + (int32_t)(min(row0 + 16 * NQ - 1, rows - 1) / a.group);
+    const int32_t hi_any = min(whi, edge), lo_any = first_seen(wlo, a.window), hi_one = min(wlo, edge), lo_one = first_seen(whi, a.window);
+
+    f4 acc[NQ][TV];
+    float mrun[NQ], lrun[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        mrun[n] = -INFINITY;
+        lrun[n] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < TV; ++t) acc[n][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    uint32_t page_ok = 0;  // whether the halves of the tile in use, and of the next, have a page (bits 0, 1 and 2, 3)
+    auto oks = [&](uint32_t t) {
+        return (uint32_t)(__builtin_amdgcn_readlane(held, (t - held_at) * 2) < a.b.pages) |
+               (uint32_t)(__builtin_amdgcn_readlane(held, (t - held_at) * 2 + 1) < a.b.pages) << 1;
+    };
+    if (t0 < t1) {
+        store(t0, lds[0][0], lds[0][1]);
+        page_ok = oks(t0);
+        if (t0 + 1 < t1) load(t0 + 1);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t t = t0; t < t1; ++t) {
+        const uint8_t *kl = lds[(t - t0) & 1][0], *vl = lds[(t - t0) & 1][1];
+        const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
+        // (a tile that none of the wave's rows sees, as at the causal edge, is passed over)
+        if (!idle & (j0 <= hi_any) & ((j0 + 31 >= lo_any) | (j0 < first))) {
+            f4 sv[NQ][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f4 x[NQ], y[NQ];  // (the small products in sums of their own)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) x[n] = y[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int st = 0; st < ST; ++st) {
+                    const h8 A = *reinterpret_cast<const h8*>(kl + ((i * ST + st) * 64 + lane) * 16);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        x[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, qh[n][st], x[n], 0, 0, 0);
+                        y[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, ql[n][st], y[n], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) sv[n][i] = (x[n] + y[n]) * qs[n];
+            }
+            const bool whole = (page_ok & 3) == 3 && j0 + 31 <= hi_one && (j0 >= lo_one || j0 + 31 < first);
+            h8 bh[NQ], bl[NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                if (!whole) {
+                    const int32_t hi_m = min(pos[n], edge), lo_m = first_seen(pos[n], a.window);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int32_t j = j0 + 16 * i + 4 * (int32_t)g + e;
+                            sv[n][i][e] = (page_ok >> i & 1) & (j <= hi_m) & ((j >= lo_m) | (j < first)) ? sv[n][i][e] : -INFINITY;
+                        }
+                }
+                float mx = fmaxf(fmaxf(fmaxf(sv[n][0][0], sv[n][0][1]), fmaxf(sv[n][0][2], sv[n][0][3])),
+                                 fmaxf(fmaxf(sv[n][1][0], sv[n][1][1]), fmaxf(sv[n][1][2], sv[n][1][3])));
+                mx = fmaxf(mrun[n], lanes4_max(mx));
+                if (__ballot(mx > mrun[n])) {
+                    const float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun[n] - mx);
+                    lrun[n] *= al;
+#pragma unroll
+                    for (int t = 0; t < TV; ++t) acc[n][t] *= al;
+                    mrun[n] = mx;
+                }
+                const float off = mrun[n] == -INFINITY ? 0.0f : mrun[n] - kProbBits;
+                uint32_t ph[4], pl[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(sv[n][i][e] - off);
+                    lrun[n] += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const _Float16 a0 = (_Float16)p[2 * e], a1 = (_Float16)p[2 * e + 1];
+                        ph[2 * i + e] = pack2(a0, a1);
+                        pl[2 * i + e] = pack2((_Float16)(p[2 * e] - (float)a0), (_Float16)(p[2 * e + 1] - (float)a1));
+                    }
+                }
+                bh[n] = __builtin_bit_cast(h8, v4u{ph[0], ph[1], ph[2], ph[3]});
+                bl[n] = __builtin_bit_cast(h8, v4u{pl[0], pl[1], pl[2], pl[3]});
+            }
+#pragma unroll
+            for (int v = 0; v < TV; ++v) {
+                const h8 A = *reinterpret_cast<const h8*>(vl + ((16 * v + m) * 4 + g) * 16);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    acc[n][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh[n], acc[n][v], 0, 0, 0);
+                    acc[n][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl[n], acc[n][v], 0, 0, 0);
+                }
+            }
+        }
+        if (t + 1 < t1) {
+            store(t + 1, lds[(t + 1 - t0) & 1][0], lds[(t + 1 - t0) & 1][1]);
+            page_ok = oks(t + 1);
+            if (t + 2 < t1) load(t + 2);
+        }
+        __syncthreads();
+    }
+    if (idle) return;
+
+    // rows to the output, or to the chunk's partial sums
+    float* part = a.part + ((size_t)(slot * a.kv_heads + h) * splits + split) * R * (W + 4);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const float l = row_total(lrun[n]);
+        float zero = l * 0.0f;
+#pragma unroll
+        for (int t = 0; t < TV; ++t) zero += (acc[n][t][0] + acc[n][t][1] + acc[n][t][2] + acc[n][t][3]) * 0.0f;
+        uint64_t odd = __ballot(!(zero == 0.0f));
+        odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;  // columns whose sums are not finite
+        const uint32_t row = row0 + 16 * n + m;
+        if (row < rows && !(odd >> m & 1)) {
             float* out = a.out + (size_t)(s.first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;
-            *reinterpret_cast<f4*>(out + x) = L == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o / L;
+            float* dst = parts == 1 ? out : part + (row - rt * R) * (W + 4);
+            const float f = parts > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            // tile t's row 4 g + e is row 16 t + 4 g + e of the transposed tile: channel E (it % (W / E)) + it / (W / E)
+            constexpr int P = W / E / 16;  // tiles per place in an octet
+#pragma unroll
+            for (int t = 0; t < P; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int d = 0; d < E; d += 4)
+                        *reinterpret_cast<f4*>(dst + E * (16 * t + 4 * g + e) + d) =
+                            f4{acc[n][d * P + t][e], acc[n][(d + 1) * P + t][e], acc[n][(d + 2) * P + t][e], acc[n][(d + 3) * P + t][e]} * f;
+            if (parts > 1 && g == 0) *reinterpret_cast<float2*>(dst + W) = make_float2(mrun[n], l);
+        }
+        for (uint32_t bad = (uint32_t)odd; bad; bad &= bad - 1) {
+            const uint32_t r = row0 + 16 * n + __builtin_ctz(bad);
+            if (r >= rows) break;
+            constexpr int EL = W / 64;
+            float q[EL], o[EL], pm, pl;
+            const size_t at = (size_t)(h * a.group + r % a.group) * W + EL * lane, token = s.first + r / a.group;
+#pragma unroll
+            for (int e = 0; e < EL; ++e) q[e] = a.q[token * a.q_stride + at + e];
+            plain_row<W, Q4, 32>(a, keys, t0, t1, 1, seq, h, s.pos0 + (int32_t)(r / a.group), s.end, q, o, pm, pl);
+            float* dst = parts == 1 ? a.out + token * a.out_stride + at : part + (r - rt * R) * (W + 4) + EL * lane;
+#pragma unroll
+            for (int e = 0; e < EL; ++e) dst[e] = parts > 1 ? o[e] : pl == 0.0f ? 0.0f : o[e] / pl;
+            if (parts > 1 && lane == 0) {  // (without the others' 2^14)
+                part[(r - rt * R) * (W + 4) + W] = pm * kLog2e + kProbBits;
+                part[(r - rt * R) * (W + 4) + W + 1] = pl;
+            }
         }
     }
 }
@@ -809,12 +1220,26 @@ hipError_t launch_kv_read(const uint8_t* k_pages, const uint8_t* v_pages, const 
     });
 }
 
-hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, const FewPlan& few, hipStream_t s) {
-    const uint32_t units = few.row_tiles * a.b.sequences * a.kv_heads;
+hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, const AttnPlan& p, hipStream_t s) {
     return by_layout(width, q4, [&](auto w, auto t) {
-        hipLaunchKernelGGL((paged_few_kernel<decltype(w)::value, decltype(t)::value>), dim3(units * few.splits), dim3(256), 0, s,
-                           a, units, few.splits, few.row_tiles, few.chunk);
-        return hipGetLastError();
+        constexpr int W = decltype(w)::value;
+        constexpr bool Q4 = decltype(t)::value;
+        const dim3 grid(p.units * p.splits), block(256);
+        if (p.rows == 16) {
+            hipLaunchKernelGGL((paged_few_kernel<W, Q4>), grid, block, 0, s, a, p.units, p.splits, p.row_tiles, p.chunk, p.join_apart);
+        } else if (p.rows == 64) {
+            hipLaunchKernelGGL((paged_many_kernel<W, Q4, 1>), grid, block, 0, s, a, p.slots, p.splits, p.chunk);
+        } else {
+            if constexpr (W <= 256)
+                hipLaunchKernelGGL((paged_many_kernel<W, Q4, 2>), grid, block, 0, s, a, p.slots, p.splits, p.chunk);
+        }
+        hipError_t e = hipGetLastError();
+        if (e == hipSuccess && p.join_apart) {
+            constexpr uint32_t C = 1024 / W < 1 ? 1 : 1024 / W;
+            hipLaunchKernelGGL(paged_join_kernel<W>, dim3(p.slots * a.kv_heads * (p.rows / C)), block, 0, s, a, p.splits, p.chunk, p.rows);
+            e = hipGetLastError();
+        }
+        return e;
     });
 }
 

@@ -269,7 +269,7 @@ int af_paged_attention_workspace(const af_paged_attention_args* p, size_t* bytes
     if (!p || !bytes) return fail(AF_ERR_INVALID, "null argument");
     const int rc = check_attention_sizes(*p);
     if (rc) return rc;
-    *bytes = kTicketBytes + few_plan(shape_of(*p)).part_bytes;
+    *bytes = kTicketBytes + attn_plan(shape_of(*p)).part_bytes;
     return AF_OK;
 }
 
@@ -299,7 +299,7 @@ int af_paged_attention(const af_paged_attention_args* p, void* stream) {
     a.b = batch_view(p->batch, p->pages);
     a.tickets = (uint32_t*)p->workspace->p;
     a.part = (float*)((char*)p->workspace->p + kTicketBytes);
-    const hipError_t e = launch_paged_attention(a, p->config.width, p->pages.type == AF_KV_Q4, few_plan(shape_of(*p)), (hipStream_t)stream);
+    const hipError_t e = launch_paged_attention(a, p->config.width, p->pages.type == AF_KV_Q4, attn_plan(shape_of(*p)), (hipStream_t)stream);
     return e == hipSuccess ? AF_OK : fail(e, "paged attention launch");
 }
 
