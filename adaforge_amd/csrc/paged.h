@@ -106,6 +106,8 @@ AF_HD uint32_t longest_tiles(const AttnShape& a, uint32_t tokens) {
     return (keys + 31) / 32;
 }
 
+constexpr uint32_t kManyRows = 64;
+
 // A launch: row tiles of `rows` rows, their keys in at most `splits` chunks of `chunk` tiles or more.  16 rows: grid
 // units (row tiles, sequences, KV heads) by splits; more: grid slots, KV heads and splits.
 struct AttnPlan {
@@ -120,7 +122,7 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     const uint64_t pairs = (uint64_t)a.sequences * a.kv_heads;  // (at most 2^22: checked by the call)
     const uint32_t tiles = longest_tiles(a, tokens);
     p.row_tiles = (uint32_t)(((uint64_t)tokens * a.group + 15) / 16);
-    p.rows = p.row_tiles > 1 ? (a.width == 512 || (uint64_t)row_slots(a, 128) * a.kv_heads < 256 ? 64 : 128) : 16;
+    p.rows = p.row_tiles > 2 ? kManyRows : 16;
     p.slots = row_slots(a, p.rows);
     if (p.row_tiles * pairs > 1u << 22) p.row_tiles = most(1, (uint32_t)((1u << 22) / pairs));
     const uint64_t sums = (uint64_t)p.slots * a.kv_heads;
@@ -133,7 +135,7 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
         splits = sums > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / sums)));
     } else {
         p.units = (uint32_t)sums;
-        splits = least(most(1, 1024 / p.units), most(1, tiles / 16));
+        splits = most(least(most(1, 256 / p.units), most(1, tiles / 8)), least(most(1, 1024 / p.units), most(1, tiles / 16)));
         splits = least(splits, 16);
     }
     p.chunk = (tiles + splits - 1) / splits;

@@ -58,13 +58,16 @@ __device__ __forceinline__ uint32_t page_of(const PagedBatch& b, uint32_t seq, i
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 // The fp16 values of a word's eight codes under scale d: pairs (2 i, 2 i + 1) at bits 4 i and 16 + 4 i.  A code n in
-// the low bits of 0x6400 is the fp16 number 1024 + n, so n - 8 is one exact subtraction, and d (n - 8) one rounding.
+// the low bits of 0x6400 is the fp16 number 1024 + n, four bits higher 1024 + 16 n, so n - 8 is one exact operation,
+// and d (n - 8) one rounding.
 __device__ __forceinline__ void unpack4(uint32_t w, _Float16 d, h2 (&o)[4]) {
+    const h2 low = {(_Float16)-1032.0f, (_Float16)-1032.0f}, high = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const h2 part = {(_Float16)0.0625f, (_Float16)0.0625f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t b = (w >> (4 * i) & 0x000F000Fu) | 0x64006400u;
-        const h2 n = __builtin_bit_cast(h2, b) - h2{(_Float16)1032.0f, (_Float16)1032.0f};
-        o[i] = n * h2{d, d};
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t v = w >> (8 * i);
+        o[2 * i] = (__builtin_bit_cast(h2, (v & 0x000F000Fu) | 0x64006400u) + low) * h2{d, d};
+        o[2 * i + 1] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (v & 0x00F000F0u) | 0x64006400u), part, high) * h2{d, d};
     }
 }
 
@@ -305,12 +308,13 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
 // base address is scalar and every load adds a constant per lane.
 //
 // fp32 rows enter as fp16 pairs hi + lo (22 bits and more): queries scaled by a power of two to below 32,
-// probabilities times 2^14, which the exponent takes in.
+// weights times 2^8, which the exponent takes in (Softmax).
 
 constexpr int kPartSC1 = 16;      // buffer access policy sc1: through to (or from) the memory side
 constexpr int kWaitVm0 = 0x0F70;  // s_waitcnt vmcnt(0), expcnt and lgkmcnt unconstrained
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kProbBits = 14.0f;
+constexpr float kProbBits = 8.0f;  // weights are held times 2^8 ..
+constexpr float kRise = 7.0f;      // .. against a maximum that may have risen by this since: below fp16's 2^16
 
 // The first key that a query at position p sees, apart from the first tokens.
 __device__ __forceinline__ int32_t first_seen(int32_t p, uint32_t window) {
@@ -328,7 +332,20 @@ __device__ __forceinline__ float lanes4_max(float v) {
     return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 
-__device__ __forceinline__ uint32_t pack2(_Float16 a, _Float16 b) { return __builtin_bit_cast(uint32_t, h2{a, b}); }
+// Two floats to nearest fp16, and x less one of them (exact: one instruction takes the fp16 operand as it is).
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, h2));
+}
+template <int HALF>
+__device__ __forceinline__ float less_half(float x, uint32_t h) {
+    float r;
+    if constexpr (HALF == 0)
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    else
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
 
 // The step and lane group whose operand holds channels 8 o .. 8 o + 7 of a key's row.
 template <int W, bool Q4>
@@ -457,6 +474,45 @@ struct VHalf {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 k[e][i] = __builtin_amdgcn_perm(x[2 * i + 1][e / 2], x[2 * i][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+    }
+};
+
+// The column's running softmax (base 2): weights 2^(score - m + kProbBits), m a maximum of the scores so far that lags
+// behind by at most kRise, so that the sums are rescaled for the first tiles and then hardly ever.
+struct Softmax {
+    float m = -INFINITY, l = 0.0f, off = 0.0f;  // l: the sum over this lane's keys; off = kProbBits - m
+
+    // Weights of the lane's eight keys, scores s (-inf: not seen) times qs, as fp16 pairs; scale(f) takes the factor of
+    // the sums so far where it is not 1 (lanes of a column agree).
+    template <typename F>
+    __device__ __forceinline__ void step(const f4 (&s)[2], float qs, h8& hi, h8& lo, F scale) {
+        const float mine = qs * fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        if (__ballot(mine > m + kRise)) {
+            const float mx = fmaxf(m, lanes4_max(mine));
+            const float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+            m = mx;
+            off = mx == -INFINITY ? 0.0f : kProbBits - mx;
+            l *= al;
+            scale(al);
+        }
+        uint32_t ph[4], pl[4];
+        float sum[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], qs, off));
+            sum[i] = (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                ph[2 * i + e] = pack_f16(p[2 * e], p[2 * e + 1]);
+                pl[2 * i + e] = pack_f16(less_half<0>(p[2 * e], ph[2 * i + e]), less_half<1>(p[2 * e + 1], ph[2 * i + e]));
+            }
+        }
+        l += sum[0] + sum[1];
+        hi = __builtin_bit_cast(h8, v4u{ph[0], ph[1], ph[2], ph[3]});
+        lo = __builtin_bit_cast(h8, v4u{pl[0], pl[1], pl[2], pl[3]});
     }
 };
 
@@ -630,25 +686,24 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         f4 acc[TV];
 #pragma unroll
         for (int t = 0; t < TV; ++t) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        float mrun = -INFINITY, lrun = 0.0f;  // (lrun: this lane's keys)
+        Softmax sm;
 #pragma unroll 1
         for (uint32_t t = t0; t < t1; t += 4) {
             const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
             const bool ok0 = ok[0], ok1 = ok[1], more = t + 4 < t1;
-            f4 sv[2];
+            f4 sv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
             uint32_t qoff = lane * 16;
             asm volatile("" : "+v"(qoff));  // (the queries stay in LDS: hoisted into registers they make the others spill)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                f4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;  // (the small products in a sum of their own)
+            for (int st = 0; st < ST; ++st) {
+                if (st % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                const h8 hi = *reinterpret_cast<const h8*>(lds + st * 2048 + qoff), lo = *reinterpret_cast<const h8*>(lds + st * 2048 + 1024 + qoff);
 #pragma unroll
-                for (int st = 0; st < ST; ++st) {
-                    if (st % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                for (int i = 0; i < 2; ++i) {
                     const h8 A = k[i].operand(st);
-                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, *reinterpret_cast<const h8*>(lds + st * 2048 + qoff), x, 0, 0, 0);
-                    y = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, *reinterpret_cast<const h8*>(lds + st * 2048 + 1024 + qoff), y, 0, 0, 0);
+                    sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, lo, sv[i], 0, 0, 0);
+                    sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, hi, sv[i], 0, 0, 0);
                 }
-                sv[i] = (x + y) * qs;
             }
             __builtin_amdgcn_sched_barrier(0);
             if (more) {
@@ -669,33 +724,11 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                         if (!(in & (j <= hi_all) & ((j >= lo_all) | (j < first)))) v[i].clear(e);
                     }
             }
-            float mx = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
-                             fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
-            mx = fmaxf(mrun, lanes4_max(mx));
-            if (__ballot(mx > mrun)) {
-                const float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun - mx);
-                lrun *= al;
+            h8 bh, bl;
+            sm.step(sv, qs, bh, bl, [&](float f) {
 #pragma unroll
-                for (int i = 0; i < TV; ++i) acc[i] *= al;
-                mrun = mx;
-            }
-            const float off = mrun == -INFINITY ? 0.0f : mrun - kProbBits;
-            uint32_t ph[4], pl[4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float p[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(sv[i][e] - off);
-                lrun += (p[0] + p[1]) + (p[2] + p[3]);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const _Float16 a0 = (_Float16)p[2 * e], a1 = (_Float16)p[2 * e + 1];
-                    ph[2 * i + e] = pack2(a0, a1);
-                    pl[2 * i + e] = pack2((_Float16)(p[2 * e] - (float)a0), (_Float16)(p[2 * e + 1] - (float)a1));
-                }
-            }
-            const h8 bh = __builtin_bit_cast(h8, v4u{ph[0], ph[1], ph[2], ph[3]});
-            const h8 bl = __builtin_bit_cast(h8, v4u{pl[0], pl[1], pl[2], pl[3]});
+                for (int i = 0; i < TV; ++i) acc[i] *= f;
+            });
             constexpr int N = TV < 8 ? TV : 8;
 #pragma unroll
             for (int o = 0; o < TV / N; ++o) {
@@ -712,7 +745,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
             }
             if (more) load_v(t + 4);
         }
-        lrun = row_total(lrun);
+        const float lrun = row_total(sm.l);
 
         // columns whose sums are not finite
         float zero = lrun * 0.0f;
@@ -727,7 +760,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         float* part = a.part + ((size_t)slot * splits + split) * 16 * (W + 4);
         __syncthreads();  // every wave is past its queries
         if (lane < 16) {
-            wm[wave][m] = mrun;
+            wm[wave][m] = sm.m;
             wl[wave][m] = lrun;
         }
 #pragma unroll 1
@@ -757,7 +790,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
 #pragma unroll
                 for (int e = 0; e < E; ++e) sums[(wave * HALFROWS + c - r0) * W + E * lane + e] = o[e];
                 if (lane == 0) {
-                    wm[wave][c] = pm * kLog2e + kProbBits;  // (its sums lack the others' 2^14)
+                    wm[wave][c] = pm * kLog2e + kProbBits;  // (its sums lack the others' factor)
                     wl[wave][c] = pl2;
                 }
             }
@@ -831,7 +864,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
 
 // ---- attention of many rows: prompts and further turns --------------------------------------------------
 //
-// Row tiles of 64 NQ rows: a wave holds 16 NQ of them from scores to output, their queries and sums in registers, and
+// Row tiles of 64 rows: a wave holds 16 of them from scores to output, their queries and sums in registers, and
 // the block's four waves share K and V through LDS, 32 keys at a time in two buffers: while one tile is used, the next
 // one is on its way (in registers, then in the other buffer) and one barrier separates tiles.  Bound by the matrix
 // cores' 8 W multiply-adds per (row, key): both operands' pairs double the 4 W of the product.
@@ -840,10 +873,23 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
 // ordered by their place in an octet (E values of a load), so that writes (lanes along octets and keys) and reads
 // (lanes along a tile's 16 rows) both sweep LDS in address order.  Q4 blocks become fp16 on the way.
 
-template <int W, bool Q4, int NQ>
-__global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(PagedAttn a, uint32_t slots, uint32_t splits,
+// The order of a product's instructions: its LDS operands are requested kAhead reads before the two products that take
+// one (left to itself the compiler requests each where it is needed, and every product waits for LDS).
+constexpr int kAhead = 4;
+template <int N>
+__device__ __forceinline__ void pipeline_operands() {
+    __builtin_amdgcn_sched_group_barrier(0x100, N < kAhead ? N : kAhead, 0);
+#pragma unroll
+    for (int f = 0; f < N; ++f) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        if (f + kAhead < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
+
+template <int W, bool Q4>
+__global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(PagedAttn a, uint32_t slots, uint32_t splits,
                                                                                 uint32_t chunk) {
-    constexpr int ST = W / 32, TV = W / 16, R = 64 * NQ;
+    constexpr int ST = W / 32, TV = W / 16, R = kManyRows;
     constexpr int E = W / 16 < 8 ? W / 16 : 8;  // channels of an octet
     constexpr int NK = Q4 ? (W + 255) / 256 : W / 64;  // a thread's pieces of K: blocks of 32 values, or octets
     constexpr int NV = (W + 255) / 256;                // and of V: four keys of an octet of channels
@@ -885,10 +931,15 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
         const uint32_t e = (tile_at(keys, min(t + lane / 2, keys.count - 1)) * 32 + lane % 2 * 16) >> a.b.page_shift;
         held = e < a.b.table_stride ? table[e] : a.b.pages;
     };
-    // the next tile's K and V on their way
+    // The next tile's K and V on their way.  Thread: pieces of K tid + 256 i, in LDS order (octets: half, step, lane; 4-bit
+    // blocks: half, block, row); of V: half, octet of channels, four keys 4 u .. 4 u + 3.  Where a half's share is whole
+    // waves (UK, UV), its address is scalar plus a constant per lane.
+    constexpr uint32_t PK = Q4 ? W : W * 4;  // pieces of K
+    constexpr bool UK = PK / 2 >= 64, UV = W / 2 >= 64;
     v4u kr[NK];
     uint32_t kd[Q4 ? NK : 1];
     uint32_t vr[NV][4][Q4 ? 1 : 4], vd[Q4 ? NV : 1][4];
+    auto half_of = [&](bool uniform, uint32_t i, uint32_t of) { return ((uniform ? wave * 64 : tid) + 256 * i) / of; };
     auto load = [&](uint32_t t) {
         if (t >= held_at + 32) pages_from(t);
         const uint32_t j0 = tile_at(keys, t) * 32;
@@ -903,32 +954,37 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
         }
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-            const uint32_t e = tid + 256 * i;
-            if constexpr (!Q4) {  // octet e: half, step, group, row
-                const uint32_t half = e / 64 / ST, st = e / 64 % ST;
-                const uint8_t* p = a.k_pages + (half ? off[1] : off[0]) + ((half ? slot_[1] : slot_[0]) + e % 16) * (W * 2) + st * 64 + e / 16 % 4 * 16;
-                kr[i] = *gp(reinterpret_cast<const v4u*>(p));
-            } else if (W >= 256 || e < W) {  // block e: half, block, row
-                const uint32_t half = e / 16 / ST, b = e / 16 % ST, sl = (half ? slot_[1] : slot_[0]) + e % 16;
-                const uint8_t* p = a.k_pages + (half ? off[1] : off[0]);
-                kr[i] = *gp(reinterpret_cast<const v4u*>(p + sl * (W / 2) + b * 16));
-                kd[i] = *gp(reinterpret_cast<const uint16_t*>(p + tokens * (W / 2) + sl * (W / 16) + b * 2));
+            const uint32_t half = half_of(UK, i, PK / 2), e = (tid + 256 * i) % (PK / 2);
+            const uint8_t* p = a.k_pages + (half ? off[1] : off[0]);
+            const uint32_t sl = half ? slot_[1] : slot_[0];
+            if constexpr (!Q4) {
+                const uint32_t st = UK ? (wave * 64 + 256 * i) % (PK / 2) / 64 : e / 64;
+                const auto* q = gp(p + (size_t)sl * (W * 2) + st * 64) + (m * (W * 2) + g * 16);
+                kr[i] = *(const __attribute__((address_space(1))) v4u*)q;
+            } else if (PK >= 256 || tid < PK) {
+                const auto* q = gp(p + (size_t)sl * (W / 2)) + (e % 16 * (W / 2) + e / 16 * 16);
+                const auto* d = gp(p + (size_t)tokens * (W / 2) + sl * (W / 16)) + (e % 16 * (W / 16) + e / 16 * 2);
+                kr[i] = *(const __attribute__((address_space(1))) v4u*)q;
+                kd[i] = *(const __attribute__((address_space(1))) uint16_t*)d;
             }
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const uint32_t e = tid + 256 * i, u = e % 8, o = e / 8;  // keys 16 (u / 4) + 4 (u % 4) .. + 3, octet o of 8 channels
-            if (W < 256 && e >= W) break;
-            const uint8_t* p = a.v_pages + (u / 4 ? off[1] : off[0]);
-            const uint32_t sl = (u / 4 ? slot_[1] : slot_[0]) + u % 4 * 4;
+            if (W < 256 && tid >= W) break;
+            const uint32_t half = half_of(UV, i, W / 2), e = (tid + 256 * i) % (W / 2), u = e % 4, o = e / 4;
+            const uint8_t* p = a.v_pages + (half ? off[1] : off[0]);
+            const uint32_t sl = half ? slot_[1] : slot_[0];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if constexpr (!Q4) {
-                    const v4u x = *gp(reinterpret_cast<const v4u*>(p + (sl + j) * (W * 2) + o * 16));
+                    const auto* q = gp(p + (size_t)sl * (W * 2)) + (u * (W * 8) + o * 16 + j * (W * 2));
+                    const v4u x = *(const __attribute__((address_space(1))) v4u*)q;
                     vr[i][j][0] = x.x, vr[i][j][1] = x.y, vr[i][j][2] = x.z, vr[i][j][3] = x.w;
                 } else {
-                    vr[i][j][0] = *gp(reinterpret_cast<const uint32_t*>(p + (sl + j) * (W / 2) + o * 4));
-                    vd[i][j] = *gp(reinterpret_cast<const uint16_t*>(p + tokens * (W / 2) + (sl + j) * (W / 16) + o / 4 * 2));
+                    const auto* q = gp(p + (size_t)sl * (W / 2)) + (u * (W * 2) + o * 4 + j * (W / 2));
+                    const auto* d = gp(p + (size_t)tokens * (W / 2) + sl * (W / 16)) + (u * (W / 4) + o / 4 * 2 + j * (W / 16));
+                    vr[i][j][0] = *(const __attribute__((address_space(1))) uint32_t*)q;
+                    vd[i][j] = *(const __attribute__((address_space(1))) uint16_t*)d;
                 }
         }
     };
@@ -939,7 +995,7 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
             const uint32_t e = tid + 256 * i;
             if constexpr (!Q4) {
                 *reinterpret_cast<v4u*>(kl + e * 16) = kr[i];
-            } else if (W >= 256 || e < W) {
+            } else if (PK >= 256 || tid < PK) {
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     h2 x[4];
@@ -952,11 +1008,24 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
         }
         const bool p0 = __builtin_amdgcn_readlane(held, (t - held_at) * 2) < a.b.pages;
         const bool p1 = __builtin_amdgcn_readlane(held, (t - held_at) * 2 + 1) < a.b.pages;
-        const bool whole = p0 & p1 & (j0 + 31 <= hi_all) & ((j0 >= lo_all) | (j0 + 31 < first));
+        if (!(p0 & p1 & (j0 + 31 <= hi_all) & ((j0 >= lo_all) | (j0 + 31 < first))))  // keys that no row sees may be anything
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t e = (tid + 256 * i) % (W / 2), half = (tid + 256 * i) / (W / 2);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int32_t key = j0 + (int32_t)(half * 16 + e % 4 * 4) + j;
+                    if (!((half ? p1 : p0) & (key <= hi_all) & ((key >= lo_all) | (key < first)))) {
+#pragma unroll
+                        for (int r = 0; r < (Q4 ? 1 : 4); ++r) vr[i][j][r] = 0;
+                        if constexpr (Q4) vd[i][j] = 0;
+                    }
+                }
+            }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const uint32_t e = tid + 256 * i, u = e % 8, o = e / 8;
-            if (W < 256 && e >= W) break;
+            if (W < 256 && tid >= W) break;
+            const uint32_t half = (tid + 256 * i) / (W / 2), e = (tid + 256 * i) % (W / 2), u = e % 4, o = e / 4;
             uint32_t x[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -970,20 +1039,12 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
                     for (int r = 0; r < 4; ++r) x[j][r] = __builtin_bit_cast(uint32_t, y[r]);
                 }
             }
-            if (!whole)  // keys that no row sees may be anything
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int32_t key = j0 + (int32_t)(u * 4) + j;
-                    if (!((u / 4 ? p1 : p0) & (key <= hi_all) & ((key >= lo_all) | (key < first))))
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) x[j][r] = 0;
-                }
-            // channel c: row (c % E) W / E + c / E of the transposed tile; piece u % 4 of 8 keys, its half u / 4
+            // channel 8 o + d: row (d % E) W / E + (8 o + d) / E of the transposed tile; its eight-key piece u, half `half`
+            uint8_t* dst = vl + (o * (8 / E) * 64 + u * 16 + half * 8);
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
                 const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
-                const uint32_t at = (d % E) * (W / E) + o * (8 / E) + d / E;
-                *reinterpret_cast<u2*>(vl + at * 64 + u % 4 * 16 + u / 4 * 8) =
+                *reinterpret_cast<u2*>(dst + ((d % E) * (W / E) + d / E) * 64) =
                     u2{__builtin_amdgcn_perm(x[1][d / 2], x[0][d / 2], sel), __builtin_amdgcn_perm(x[3][d / 2], x[2][d / 2], sel)};
             }
         }
@@ -994,15 +1055,12 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
     }
 
     // the queries: lane (column m, g) holds channels 32 s + 8 g .. + 7 of step s, as scaled fp16 pairs
-    h8 qh[NQ][ST], ql[NQ][ST];
-    float qs[NQ];
-    int32_t pos[NQ];
-    const uint32_t row0 = rt * R + wave * (16 * NQ);
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const uint32_t row = min(row0 + 16 * n + m, rows - 1);  // (columns past the last row: as the last)
-        const float* src = a.q + (size_t)(s.first + row / a.group) * a.q_stride + (size_t)(h * a.group + row % a.group) * W + 8 * g;
-        pos[n] = s.pos0 + (int32_t)(row / a.group);
+    h8 qh[ST], ql[ST];
+    float qs;
+    const uint32_t row0 = rt * R + wave * 16, row = row0 + m, real = min(row, rows - 1);  // (columns past the last row: as the last)
+    const int32_t pos = s.pos0 + (int32_t)(real / a.group);
+    {
+        const float* src = a.q + (size_t)(s.first + real / a.group) * a.q_stride + (size_t)(h * a.group + real % a.group) * W + 8 * g;
         float mx = 0.0f;
 #pragma unroll
         for (int st = 0; st < ST; ++st)
@@ -1013,7 +1071,7 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[e]));
             }
         const float up = query_scale(lanes4_max(mx));
-        qs[n] = a.scale / up * kLog2e;
+        qs = a.scale / up * kLog2e;
 #pragma unroll
         for (int st = 0; st < ST; ++st)
 #pragma unroll
@@ -1022,26 +1080,22 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float y = x[e] * up;
-                    qh[n][st][4 * i + e] = (_Float16)y;
-                    ql[n][st][4 * i + e] = (_Float16)(y - (float)qh[n][st][4 * i + e]);
+                    qh[st][4 * i + e] = (_Float16)y;
+                    ql[st][4 * i + e] = (_Float16)(y - (float)qh[st][4 * i + e]);
                 }
             }
     }
     // this wave's rows: what any and what every one of them sees
     const bool idle = row0 >= rows;
     const int32_t wlo = s.pos0 + (int32_t)(min(row0, rows - 1) / a.group);
-    const int32_t whi = s.pos0 + (int32_t)(min(row0 + 16 * NQ - 1, rows - 1) / a.group);
+    const int32_t whi = s.pos0 + (int32_t)(min(row0 + 15, rows - 1) / a.group);
     const int32_t hi_any = min(whi, edge), lo_any = first_seen(wlo, a.window), hi_one = min(wlo, edge), lo_one = first_seen(whi, a.window);
+    const int32_t hi_m = min(pos, edge), lo_m = first_seen(pos, a.window);
 
-    f4 acc[NQ][TV];
-    float mrun[NQ], lrun[NQ];
+    f4 acc[TV];
+    Softmax sm;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        mrun[n] = -INFINITY;
-        lrun[n] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < TV; ++t) acc[n][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int t = 0; t < TV; ++t) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     uint32_t page_ok = 0;  // whether the halves of the tile in use, and of the next, have a page (bits 0, 1 and 2, 3)
     auto oks = [&](uint32_t t) {
         return (uint32_t)(__builtin_amdgcn_readlane(held, (t - held_at) * 2) < a.b.pages) |
@@ -1059,75 +1113,36 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
         const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
         // (a tile that none of the wave's rows sees, as at the causal edge, is passed over)
         if (!idle & (j0 <= hi_any) & ((j0 + 31 >= lo_any) | (j0 < first))) {
-            f4 sv[NQ][2];
+            f4 sv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                f4 x[NQ], y[NQ];  // (the small products in sums of their own)
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) x[n] = y[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int st = 0; st < ST; ++st) {
-                    const h8 A = *reinterpret_cast<const h8*>(kl + ((i * ST + st) * 64 + lane) * 16);
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        x[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, qh[n][st], x[n], 0, 0, 0);
-                        y[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, ql[n][st], y[n], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) sv[n][i] = (x[n] + y[n]) * qs[n];
+            for (int f = 0; f < 2 * ST; ++f) {
+                const int i = f & 1, st = f >> 1;
+                const h8 A = *reinterpret_cast<const h8*>(kl + ((i * ST + st) * 64 + lane) * 16);
+                sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, ql[st], sv[i], 0, 0, 0);
+                sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, qh[st], sv[i], 0, 0, 0);
             }
+            pipeline_operands<2 * ST>();
             const bool whole = (page_ok & 3) == 3 && j0 + 31 <= hi_one && (j0 >= lo_one || j0 + 31 < first);
-            h8 bh[NQ], bl[NQ];
+            if (!whole)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                if (!whole) {
-                    const int32_t hi_m = min(pos[n], edge), lo_m = first_seen(pos[n], a.window);
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int32_t j = j0 + 16 * i + 4 * (int32_t)g + e;
-                            sv[n][i][e] = (page_ok >> i & 1) & (j <= hi_m) & ((j >= lo_m) | (j < first)) ? sv[n][i][e] : -INFINITY;
-                        }
-                }
-                float mx = fmaxf(fmaxf(fmaxf(sv[n][0][0], sv[n][0][1]), fmaxf(sv[n][0][2], sv[n][0][3])),
-                                 fmaxf(fmaxf(sv[n][1][0], sv[n][1][1]), fmaxf(sv[n][1][2], sv[n][1][3])));
-                mx = fmaxf(mrun[n], lanes4_max(mx));
-                if (__ballot(mx > mrun[n])) {
-                    const float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mrun[n] - mx);
-                    lrun[n] *= al;
-#pragma unroll
-                    for (int t = 0; t < TV; ++t) acc[n][t] *= al;
-                    mrun[n] = mx;
-                }
-                const float off = mrun[n] == -INFINITY ? 0.0f : mrun[n] - kProbBits;
-                uint32_t ph[4], pl[4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(sv[n][i][e] - off);
-                    lrun[n] += (p[0] + p[1]) + (p[2] + p[3]);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const _Float16 a0 = (_Float16)p[2 * e], a1 = (_Float16)p[2 * e + 1];
-                        ph[2 * i + e] = pack2(a0, a1);
-                        pl[2 * i + e] = pack2((_Float16)(p[2 * e] - (float)a0), (_Float16)(p[2 * e + 1] - (float)a1));
+                    for (int e = 0; e < 4; ++e) {
+                        const int32_t j = j0 + 16 * i + 4 * (int32_t)g + e;
+                        sv[i][e] = (page_ok >> i & 1) & (j <= hi_m) & ((j >= lo_m) | (j < first)) ? sv[i][e] : -INFINITY;
                     }
-                }
-                bh[n] = __builtin_bit_cast(h8, v4u{ph[0], ph[1], ph[2], ph[3]});
-                bl[n] = __builtin_bit_cast(h8, v4u{pl[0], pl[1], pl[2], pl[3]});
-            }
+            h8 bh, bl;
+            sm.step(sv, qs, bh, bl, [&](float f) {
+#pragma unroll
+                for (int v = 0; v < TV; ++v) acc[v] *= f;
+            });
 #pragma unroll
             for (int v = 0; v < TV; ++v) {
                 const h8 A = *reinterpret_cast<const h8*>(vl + ((16 * v + m) * 4 + g) * 16);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    acc[n][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh[n], acc[n][v], 0, 0, 0);
-                    acc[n][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl[n], acc[n][v], 0, 0, 0);
-                }
+                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[v], 0, 0, 0);
+                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[v], 0, 0, 0);
             }
+            pipeline_operands<TV>();
         }
         if (t + 1 < t1) {
             store(t + 1, lds[(t + 1 - t0) & 1][0], lds[(t + 1 - t0) & 1][1]);
@@ -1140,47 +1155,43 @@ __global__ __launch_bounds__(256, W * NQ >= 512 ? 1 : 2) void paged_many_kernel(
 
     // rows to the output, or to the chunk's partial sums
     float* part = a.part + ((size_t)(slot * a.kv_heads + h) * splits + split) * R * (W + 4);
+    const float l = row_total(sm.l);
+    float zero = l * 0.0f;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const float l = row_total(lrun[n]);
-        float zero = l * 0.0f;
+    for (int t = 0; t < TV; ++t) zero += (acc[t][0] + acc[t][1] + acc[t][2] + acc[t][3]) * 0.0f;
+    uint64_t odd = __ballot(!(zero == 0.0f));
+    odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;  // columns whose sums are not finite
+    if (row < rows && !(odd >> m & 1)) {
+        float* out = a.out + (size_t)(s.first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;
+        float* dst = parts == 1 ? out : part + (row - rt * R) * (W + 4);
+        const float f = parts > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        // tile t's row 4 g + e is row 16 t + 4 g + e of the transposed tile: channel E (it % (W / E)) + it / (W / E)
+        constexpr int P = W / E / 16;  // tiles per place in an octet
 #pragma unroll
-        for (int t = 0; t < TV; ++t) zero += (acc[n][t][0] + acc[n][t][1] + acc[n][t][2] + acc[n][t][3]) * 0.0f;
-        uint64_t odd = __ballot(!(zero == 0.0f));
-        odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;  // columns whose sums are not finite
-        const uint32_t row = row0 + 16 * n + m;
-        if (row < rows && !(odd >> m & 1)) {
-            float* out = a.out + (size_t)(s.first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;
-            float* dst = parts == 1 ? out : part + (row - rt * R) * (W + 4);
-            const float f = parts > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            // tile t's row 4 g + e is row 16 t + 4 g + e of the transposed tile: channel E (it % (W / E)) + it / (W / E)
-            constexpr int P = W / E / 16;  // tiles per place in an octet
+        for (int t = 0; t < P; ++t)
 #pragma unroll
-            for (int t = 0; t < P; ++t)
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int d = 0; d < E; d += 4)
+                    *reinterpret_cast<f4*>(dst + E * (16 * t + 4 * g + e) + d) =
+                        f4{acc[d * P + t][e], acc[(d + 1) * P + t][e], acc[(d + 2) * P + t][e], acc[(d + 3) * P + t][e]} * f;
+        if (parts > 1 && g == 0) *reinterpret_cast<float2*>(dst + W) = make_float2(sm.m, l);
+    }
+    for (uint32_t bad = (uint32_t)odd; bad; bad &= bad - 1) {
+        const uint32_t r = row0 + __builtin_ctz(bad);
+        if (r >= rows) break;
+        constexpr int EL = W / 64;
+        float q[EL], o[EL], pm, pl;
+        const size_t at = (size_t)(h * a.group + r % a.group) * W + EL * lane, token = s.first + r / a.group;
 #pragma unroll
-                    for (int d = 0; d < E; d += 4)
-                        *reinterpret_cast<f4*>(dst + E * (16 * t + 4 * g + e) + d) =
-                            f4{acc[n][d * P + t][e], acc[n][(d + 1) * P + t][e], acc[n][(d + 2) * P + t][e], acc[n][(d + 3) * P + t][e]} * f;
-            if (parts > 1 && g == 0) *reinterpret_cast<float2*>(dst + W) = make_float2(mrun[n], l);
-        }
-        for (uint32_t bad = (uint32_t)odd; bad; bad &= bad - 1) {
-            const uint32_t r = row0 + 16 * n + __builtin_ctz(bad);
-            if (r >= rows) break;
-            constexpr int EL = W / 64;
-            float q[EL], o[EL], pm, pl;
-            const size_t at = (size_t)(h * a.group + r % a.group) * W + EL * lane, token = s.first + r / a.group;
+        for (int e = 0; e < EL; ++e) q[e] = a.q[token * a.q_stride + at + e];
+        plain_row<W, Q4, 32>(a, keys, t0, t1, 1, seq, h, s.pos0 + (int32_t)(r / a.group), s.end, q, o, pm, pl);
+        float* dst = parts == 1 ? a.out + token * a.out_stride + at : part + (r - rt * R) * (W + 4) + EL * lane;
 #pragma unroll
-            for (int e = 0; e < EL; ++e) q[e] = a.q[token * a.q_stride + at + e];
-            plain_row<W, Q4, 32>(a, keys, t0, t1, 1, seq, h, s.pos0 + (int32_t)(r / a.group), s.end, q, o, pm, pl);
-            float* dst = parts == 1 ? a.out + token * a.out_stride + at : part + (r - rt * R) * (W + 4) + EL * lane;
-#pragma unroll
-            for (int e = 0; e < EL; ++e) dst[e] = parts > 1 ? o[e] : pl == 0.0f ? 0.0f : o[e] / pl;
-            if (parts > 1 && lane == 0) {  // (without the others' 2^14)
-                part[(r - rt * R) * (W + 4) + W] = pm * kLog2e + kProbBits;
-                part[(r - rt * R) * (W + 4) + W + 1] = pl;
-            }
+        for (int e = 0; e < EL; ++e) dst[e] = parts > 1 ? o[e] : pl == 0.0f ? 0.0f : o[e] / pl;
+        if (parts > 1 && lane == 0) {  // (without the others' factor)
+            part[(r - rt * R) * (W + 4) + W] = pm * kLog2e + kProbBits;
+            part[(r - rt * R) * (W + 4) + W + 1] = pl;
         }
     }
 }
@@ -1227,11 +1238,8 @@ hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, c
         const dim3 grid(p.units * p.splits), block(256);
         if (p.rows == 16) {
             hipLaunchKernelGGL((paged_few_kernel<W, Q4>), grid, block, 0, s, a, p.units, p.splits, p.row_tiles, p.chunk, p.join_apart);
-        } else if (p.rows == 64) {
-            hipLaunchKernelGGL((paged_many_kernel<W, Q4, 1>), grid, block, 0, s, a, p.slots, p.splits, p.chunk);
         } else {
-            if constexpr (W <= 256)
-                hipLaunchKernelGGL((paged_many_kernel<W, Q4, 2>), grid, block, 0, s, a, p.slots, p.splits, p.chunk);
+            hipLaunchKernelGGL((paged_many_kernel<W, Q4>), grid, block, 0, s, a, p.slots, p.splits, p.chunk);
         }
         hipError_t e = hipGetLastError();
         if (e == hipSuccess && p.join_apart) {
