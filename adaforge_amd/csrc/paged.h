@@ -141,7 +141,7 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     p.chunk = (tiles + splits - 1) / splits;
     p.splits = (tiles + p.chunk - 1) / p.chunk;
     const uint64_t row_bytes = (uint64_t)(a.width + 4) * 4;
-    p.join_apart = p.splits > 1 && (p.rows > 16 || p.splits * least(16, tokens * a.group) * row_bytes > 65536);
+    p.join_apart = p.splits > 1 && (p.rows > 16 || p.splits * least(16, tokens * a.group) * row_bytes > 131072);
     p.part_bytes = p.splits > 1 ? (size_t)(sums * p.splits * p.rows * row_bytes) : 0;
     return p;
 }
@@ -201,11 +201,9 @@ hipError_t launch_logits_select(const LogitsSelect& a, hipStream_t s);
 
 #endif
 
-// Tokens of a row's slice in the choice of a token, and the slices of a row.
+// The choice of a token: a block takes a slice of a row: 4,096 tokens where that makes 1,024 blocks and more, else 1,024.
 AF_HD uint32_t logits_slice(uint32_t rows, uint32_t vocabulary) {
-    (void)rows;
-    (void)vocabulary;
-    return 4096;
+    return (uint64_t)rows * vocabulary >= (uint64_t)4096 * 1024 ? 4096 : 1024;
 }
 
 }  // namespace af

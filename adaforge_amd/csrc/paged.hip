@@ -26,9 +26,24 @@ __device__ __forceinline__ uint32_t last_sequence(uint32_t sequences, F before) 
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// The sequence whose rows hold row `token`.
-__device__ __forceinline__ uint32_t sequence_of(const PagedBatch& b, uint32_t token) {
-    return last_sequence(b.sequences, [&](uint32_t s) { return b.starts[s] <= token; });
+// The last sequence with before(start, s) true, and its span: one round of loads for up to 64 sequences.  meanwhile()
+// is called once the first loads are on their way.
+template <typename F, typename G>
+__device__ __forceinline__ uint32_t find_span(const PagedBatch& b, F before, Span& s, G meanwhile) {
+    if (b.sequences <= 64) {
+        const uint32_t i = min(threadIdx.x & 63, b.sequences - 1);
+        const uint32_t start = *gp(b.starts + i), stop = *gp(b.starts + i + 1), length = *gp(b.lengths + i);
+        __builtin_amdgcn_sched_barrier(0);
+        meanwhile();
+        const uint64_t at = __ballot((threadIdx.x & 63) < b.sequences && before(start, i));
+        const uint32_t seq = __builtin_amdgcn_readfirstlane(max(1, __popcll(at)) - 1);
+        s = span_of(__builtin_amdgcn_readlane(start, seq), __builtin_amdgcn_readlane(stop, seq), __builtin_amdgcn_readlane(length, seq), b);
+        return seq;
+    }
+    meanwhile();
+    const uint32_t seq = last_sequence(b.sequences, [&](uint32_t k) { return before(b.starts[k], k); });
+    s = span_of(b.starts[seq], b.starts[seq + 1], b.lengths[seq], b);
+    return seq;
 }
 
 struct Place {
@@ -37,10 +52,11 @@ struct Place {
     bool row;  // the row belongs to a sequence
 };
 
-__device__ __forceinline__ Place place_of(const PagedBatch& b, uint32_t token) {
+template <typename G>
+__device__ __forceinline__ Place place_of(const PagedBatch& b, uint32_t token, G meanwhile) {
     Place p;
-    p.seq = sequence_of(b, token);
-    const Span s = span_of(b.starts[p.seq], b.starts[p.seq + 1], b.lengths[p.seq], b);
+    Span s;
+    p.seq = find_span(b, [&](uint32_t start, uint32_t) { return start <= token; }, s, meanwhile);
     p.row = token >= s.first && token - s.first < s.count;
     p.pos = s.pos0 + (int32_t)(token - s.first);
     return p;
@@ -61,139 +77,172 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 // the low bits of 0x6400 is the fp16 number 1024 + n, four bits higher 1024 + 16 n, so n - 8 is one exact operation,
 // and d (n - 8) one rounding.
 __device__ __forceinline__ void unpack4(uint32_t w, _Float16 d, h2 (&o)[4]) {
+    // (one instruction each; from w & mask | magic the compiler makes two)
+    auto code = [](uint32_t v, uint32_t mask) {
+        uint32_t r;
+        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(v), "s"(mask), "v"(0x64006400u));
+        return __builtin_bit_cast(h2, r);
+    };
     const h2 low = {(_Float16)-1032.0f, (_Float16)-1032.0f}, high = {(_Float16)-72.0f, (_Float16)-72.0f};
     const h2 part = {(_Float16)0.0625f, (_Float16)0.0625f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const uint32_t v = w >> (8 * i);
-        o[2 * i] = (__builtin_bit_cast(h2, (v & 0x000F000Fu) | 0x64006400u) + low) * h2{d, d};
-        o[2 * i + 1] = __builtin_elementwise_fma(__builtin_bit_cast(h2, (v & 0x00F000F0u) | 0x64006400u), part, high) * h2{d, d};
+        o[2 * i] = (code(v, 0x000F000Fu) + low) * h2{d, d};
+        o[2 * i + 1] = __builtin_elementwise_fma(code(v, 0x00F000F0u), part, high) * h2{d, d};
     }
 }
 
 // ---- append -----------------------------------------------------------------------------------------
 //
-// A wave takes one head's row of a token: its sum of squares in 64 bits, then each pair's rotation, one rounding to
+// A wave takes N heads' rows of a token: their sums of squares in 64 bits, then each pair's rotation, one rounding to
 // f32, and for K and V the cache's type.  An angle is position times turns mod 2^64 as a fraction of a turn: a
 // product that wraps keeps exactly the part that sine and cosine see, so far positions lose nothing and no general
-// argument reduction is needed.
+// argument reduction is needed.  Its rows are on their way while the token's place is looked up.  N = 4 shares the sines
+// among four rows and keeps four times the bytes in flight; N = 1 spreads a decode step over the chip.
 
-template <int W, bool Q4>
+template <int W, bool Q4, int N>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppend a, uint32_t groups, uint32_t tasks) {
     constexpr int P = W / 128 ? W / 128 : 1, HALF = W / 2;  // pairs per lane
-    __shared__ __align__(16) float rows[4][W];
+    __shared__ __align__(16) float rows[Q4 ? 4 : 1][Q4 ? W : 4];
     const uint32_t lane = threadIdx.x & 63, wave = wave_id(), heads = a.q_heads + 2 * a.kv_heads;
+    const bool on = (int)lane * P < HALF;
     for (uint32_t task = blockIdx.x; task < tasks; task += gridDim.x) {
-        const uint32_t token = task / groups, r = task % groups * 4 + wave;
-        if (r >= heads) continue;
-        const Place at = place_of(a.b, token);
+        const uint32_t token = task / groups, r0 = (task % groups * 4 + wave) * N;
+        if (r0 >= heads) continue;
+        float x[N][2][P];
+        uint64_t turn_of[P];
+        const bool turned = a.turns && r0 < a.q_heads + a.kv_heads;
+        const Place at = place_of(a.b, token, [&] {
+            if (turned && on)
+#pragma unroll
+                for (int i = 0; i < P; ++i) turn_of[i] = a.turns[lane * P + i];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const uint32_t r = min(r0 + k, heads - 1);
+                const float* src = r < a.q_heads                  ? a.q + (size_t)token * a.q_stride + (size_t)r * W
+                                   : r >= a.q_heads + a.kv_heads ? a.v + (size_t)token * a.v_stride + (size_t)(r - a.q_heads - a.kv_heads) * W
+                                                                 : a.k + (size_t)token * a.k_stride + (size_t)(r - a.q_heads) * W;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < P; ++i) x[k][h][i] = on ? src[h * HALF + lane * P + i] : 0.0f;
+            }
+        });
         if (!at.row) continue;
-        const bool is_q = r < a.q_heads, is_v = r >= a.q_heads + a.kv_heads;
-        const uint32_t head = is_q ? r : is_v ? r - a.q_heads - a.kv_heads : r - a.q_heads;
-        const float* src = is_q ? a.q + (size_t)token * a.q_stride
-                                : is_v ? a.v + (size_t)token * a.v_stride : a.k + (size_t)token * a.k_stride;
-        src += (size_t)head * W;
-        const float* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
-        const float eps = is_q ? a.q_eps : is_v ? a.v_eps : a.k_eps;
-        const bool norm = is_v ? a.v_norm != 0 : w != nullptr, on = (int)lane * P < HALF;
-        float x[2][P];
-        double ss = 0.0;
+        const uint32_t page = page_of(a.b, at.seq, at.pos), tokens = 1u << a.b.page_shift, slot = (uint32_t)at.pos & (tokens - 1);
+        double sn[P], cs[P];
+        if (turned && on)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < P; ++i)
+                sincospi((double)(int64_t)((uint64_t)(int64_t)at.pos * turn_of[i]) * 0x1p-63, &sn[i], &cs[i]);
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                x[h][i] = on ? src[h * HALF + lane * P + i] : 0.0f;
-                ss = __fma_rn((double)x[h][i], (double)x[h][i], ss);
-            }
-        const double rn = norm ? inv_rms(wave_sum(ss), W, eps) : 1.0;
-        const uint64_t* turns = is_v ? nullptr : a.turns;
-        float y[2][P];
-        if (on) {
+        for (int k = 0; k < N; ++k) {
+            const uint32_t r = r0 + k;
+            if (r >= heads) break;
+            const bool is_q = r < a.q_heads, is_v = r >= a.q_heads + a.kv_heads;
+            const uint32_t head = is_q ? r : is_v ? r - a.q_heads - a.kv_heads : r - a.q_heads;
+            const float* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+            const bool norm = is_v ? a.v_norm != 0 : w != nullptr, turn = turned && !is_v;
+            float y[2][P];
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int c = lane * P + i;
-                double u = (double)x[0][i], v = (double)x[1][i];
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < P; ++i) y[h][i] = x[k][h][i];
+            if (norm || turn) {
+                double rn = 1.0;
                 if (norm) {
-                    u *= rn;
-                    v *= rn;
+                    double ss = 0.0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < P; ++i) ss = __fma_rn((double)x[k][h][i], (double)x[k][h][i], ss);
+                    const float eps = is_q ? a.q_eps : is_v ? a.v_eps : a.k_eps;
+                    ss = wave_sum(ss);
+                    rn = ss < 1e300 ? inv_rms_fast(ss, W, eps) : inv_rms(ss, W, eps);  // (an infinite row: 0, as divided)
                 }
-                if (w) {
-                    u *= (double)w[c];
-                    v *= (double)w[HALF + c];
-                }
-                if (turns) {
-                    const int64_t t = (int64_t)((uint64_t)(int64_t)at.pos * turns[c]);
-                    double sn, cs;
-                    sincospi((double)t * 0x1p-63, &sn, &cs);
-                    const double u1 = u * cs - v * sn;
-                    v = u * sn + v * cs;
-                    u = u1;
-                }
-                y[0][i] = (float)u;
-                y[1][i] = (float)v;
+                if (on)
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        const int c = lane * P + i;
+                        double u = (double)x[k][0][i], v = (double)x[k][1][i];
+                        if (norm) {
+                            u *= rn;
+                            v *= rn;
+                        }
+                        if (w) {
+                            u *= (double)w[c];
+                            v *= (double)w[HALF + c];
+                        }
+                        if (turn) {
+                            const double u1 = u * cs[i] - v * sn[i];
+                            v = u * sn[i] + v * cs[i];
+                            u = u1;
+                        }
+                        y[0][i] = (float)u;
+                        y[1][i] = (float)v;
+                    }
             }
-        }
-        if (is_q) {
-            float* dst = a.q_out + (size_t)token * a.q_out_stride + (size_t)head * W;
-            if (on)
+            if (is_q) {
+                float* dst = a.q_out + (size_t)token * a.q_out_stride + (size_t)head * W;
+                if (on)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < P; ++i) dst[h * HALF + lane * P + i] = y[h][i];
-            continue;
-        }
-        const uint32_t page = page_of(a.b, at.seq, at.pos);
-        if (page >= a.b.pages) continue;
-        const uint32_t tokens = 1u << a.b.page_shift, slot = (uint32_t)at.pos & (tokens - 1);
-        uint8_t* dst = (is_v ? a.v_pages : a.k_pages) +
-                       ((size_t)page * a.kv_heads + head) * page_part_bytes(Q4, tokens, W);
-        if constexpr (!Q4) {
-            uint16_t* d16 = reinterpret_cast<uint16_t*>(dst) + (size_t)slot * W;
-            if (on)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < P; ++i) d16[h * HALF + lane * P + i] = f2h(y[h][i]);
-        } else {
-            // through the wave's own LDS row: lane c then holds values 8 c .. 8 c + 7, four lanes a block
-            if (on)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < P; ++i) rows[wave][h * HALF + lane * P + i] = y[h][i];
-            __builtin_amdgcn_wave_barrier();
-            if (lane < W / 8) {
-                float e[8], high = -INFINITY, low = INFINITY;
-                bool bad = false;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    e[i] = rows[wave][8 * lane + i];
-                    high = fmaxf(high, e[i]);
-                    low = fminf(low, e[i]);
-                    bad |= !(fabsf(e[i]) < INFINITY);
-                }
-#pragma unroll
-                for (int s = 1; s < 4; s <<= 1) {
-                    high = fmaxf(high, __shfl_xor(high, s));
-                    low = fminf(low, __shfl_xor(low, s));
-                    bad |= __shfl_xor((int)bad, s) != 0;
-                }
-                uint16_t d = f2h((high >= -low ? high : low) / -8.0f);
-                if (bad || (d & 0x7C00) == 0x7C00) d = 0x7E00;  // not finite: the block stands for NaNs
-                const double scale = (double)h2f(d);
-                uint32_t word = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const double n = scale == 0.0 || (d & 0x7C00) == 0x7C00
-                                         ? 8.0
-                                         : fmin(fmax(rint((double)e[i] / scale) + 8.0, 0.0), 15.0);
-                    word |= (uint32_t)n << (4 * (i / 2) + 16 * (i & 1));
-                }
-                reinterpret_cast<uint32_t*>(dst)[(size_t)slot * (W / 8) + lane] = word;
-                if (lane % 4 == 0)
-                    reinterpret_cast<uint16_t*>(dst + (size_t)tokens * (W / 2))[slot * (W / 32) + lane / 4] = d;
+                        for (int i = 0; i < P; ++i) dst[h * HALF + lane * P + i] = y[h][i];
+                continue;
             }
-            __builtin_amdgcn_wave_barrier();
+            if (page >= a.b.pages) continue;
+            uint8_t* dst = (is_v ? a.v_pages : a.k_pages) +
+                           ((size_t)page * a.kv_heads + head) * page_part_bytes(Q4, tokens, W);
+            if constexpr (!Q4) {
+                uint16_t* d16 = reinterpret_cast<uint16_t*>(dst) + (size_t)slot * W;
+                if (on)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < P; ++i) d16[h * HALF + lane * P + i] = f2h(y[h][i]);
+            } else {
+                // through the wave's own LDS row: lane c then holds values 8 c .. 8 c + 7, four lanes a block
+                if (on)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < P; ++i) rows[wave][h * HALF + lane * P + i] = y[h][i];
+                __builtin_amdgcn_wave_barrier();
+                if (lane < W / 8) {
+                    float e[8], high = -INFINITY, low = INFINITY;
+                    bool bad = false;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        e[i] = rows[wave][8 * lane + i];
+                        high = fmaxf(high, e[i]);
+                        low = fminf(low, e[i]);
+                        bad |= !(fabsf(e[i]) < INFINITY);
+                    }
+                    high = fmaxf(high, dpp<kDppXor1>(high));
+                    high = fmaxf(high, dpp<kDppXor2>(high));
+                    low = fminf(low, dpp<kDppXor1>(low));
+                    low = fminf(low, dpp<kDppXor2>(low));
+                    float odd = bad ? 1.0f : 0.0f;
+                    odd = fmaxf(odd, dpp<kDppXor1>(odd));
+                    odd = fmaxf(odd, dpp<kDppXor2>(odd));
+                    uint16_t d = f2h((high >= -low ? high : low) / -8.0f);
+                    if (odd != 0.0f || (d & 0x7C00) == 0x7C00) d = 0x7E00;  // not finite: the block stands for NaNs
+                    const bool plain = d != 0x7E00 && (d & 0x7FFF) != 0;
+                    const double scale = (double)h2f(d);
+                    uint32_t word = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const double n = plain ? fmin(fmax(rint((double)e[i] / scale) + 8.0, 0.0), 15.0) : 8.0;
+                        word |= (uint32_t)n << (4 * (i / 2) + 16 * (i & 1));
+                    }
+                    reinterpret_cast<uint32_t*>(dst)[(size_t)slot * (W / 8) + lane] = word;
+                    if (lane % 4 == 0)
+                        reinterpret_cast<uint16_t*>(dst + (size_t)tokens * (W / 2))[slot * (W / 32) + lane / 4] = d;
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
         }
     }
 }
@@ -217,7 +266,7 @@ template <int W, bool Q4>
 __global__ __launch_bounds__(256) void kv_read_kernel(const uint8_t* k_pages, const uint8_t* v_pages, PagedBatch b,
                                                       uint32_t kv_heads, uint16_t* k, uint16_t* v) {
     for (uint32_t token = blockIdx.x; token < b.tokens; token += gridDim.x) {
-        const Place at = place_of(b, token);
+        const Place at = place_of(b, token, [] {});
         if (!at.row) continue;
         const uint32_t page = page_of(b, at.seq, at.pos), tokens = 1u << b.page_shift, slot = (uint32_t)at.pos & (tokens - 1);
         const uint32_t n = kv_heads * (W / 8);
@@ -522,43 +571,68 @@ __device__ __forceinline__ void chunks_of(uint32_t tiles, uint32_t chunk, uint32
     parts = max(1u, (tiles + len - 1) / len);
 }
 
-// Adds sums (o, L) of maximum m to those of maximum M, as weights 2^m; a chunk that saw nothing has m = -inf, l = 0.
-__device__ __forceinline__ void join(f4& o, float& L, float& M, const f4& v, float l, float m) {
-    if (m == -INFINITY && l == 0.0f) return;
-    const float mn = fmaxf(M, m);
-    const float al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(m - mn);
-    const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};  // (no infinity times a zero weight)
-    L = L * al + l * f;
-    o = (al == 0.0f ? zero : o * al) + (f == 0.0f ? zero : v * f);
-    M = mn;
-}
-
-// Rows [c0, nr) of a row tile from its chunks' partial sums, [parts][R][W + 4], every nth quad of channels by a thread.
+// Rows c0, c0 + 4, .. of a row tile from its chunks' partial sums [parts][R][W + 4] (sums, maximum, sum of weights), a
+// row per wave: the chunks' weights first, a chunk per lane, then their sums, eight loads of a lane in flight and
+// in the order of the chunks.  parts: at most 128.
 template <int W>
 __device__ __forceinline__ void join_parts(const PagedAttn& a, const float* part, uint32_t splits, uint32_t parts, uint32_t R,
                                            uint32_t c0, uint32_t nr, uint32_t row0, uint32_t first, uint32_t h) {
+    constexpr uint32_t L = W / 4 < 64 ? W / 4 : 64, G = 64 / L, K = W / 4 / L;  // lanes of a row, chunks side by side, quads of a lane
+    constexpr uint32_t U = 8 / K;                                               // chunks of a lane in flight
     const __amdgpu_buffer_rsrc_t rs =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, (int)(splits * R * (W + 4) * 4), 0x00020000);
-    for (uint32_t i = threadIdx.x; i < (nr - c0) * (W / 4); i += 256) {
-        const uint32_t c = c0 + i / (W / 4), x = i % (W / 4) * 4, row = row0 + c;
-        float M = -INFINITY, L = 0.0f;
-        f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t p0 = 0; p0 < parts; p0 += 8) {
-            u2 ml[8];
-            v4u sv[8];
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t c = c0 + wave_id(); c < nr; c += 4) {
+        v4u v[U][K];
+        auto load = [&](uint32_t q0) {
 #pragma unroll
-            for (uint32_t u = 0; u < 8; ++u) {
-                const uint32_t at = (min(p0 + u, parts - 1) * R + c) * (W + 4);
-                ml[u] = __builtin_amdgcn_raw_buffer_load_b64(rs, (at + W) * 4, 0, kPartSC1);
-                sv[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, (at + x) * 4, 0, kPartSC1);
-            }
+            for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
-            for (uint32_t u = 0; u < 8; ++u)
-                if (p0 + u < parts)
-                    join(o, L, M, __builtin_bit_cast(f4, sv[u]), __uint_as_float(ml[u].y), __uint_as_float(ml[u].x));
+                for (uint32_t k = 0; k < K; ++k)
+                    v[u][k] = __builtin_amdgcn_raw_buffer_load_b128(
+                        rs, ((min(q0 + lane / L + u * G, parts - 1) * R + c) * (W + 4) + (lane % L + L * k) * 4) * 4, 0, kPartSC1);
+        };
+        u2 ml[2];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i)
+            ml[i] = __builtin_amdgcn_raw_buffer_load_b64(rs, ((min(lane + 64 * i, parts - 1) * R + c) * (W + 4) + W) * 4, 0, kPartSC1);
+        load(0);
+        float m[2], l[2];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            m[i] = lane + 64 * i < parts ? __uint_as_float(ml[i].x) : -INFINITY;
+            l[i] = lane + 64 * i < parts ? __uint_as_float(ml[i].y) : 0.0f;
         }
+        const float M = wave_max(fmaxf(m[0], m[1]));
+        float f[2];  // (a chunk that saw nothing has maximum -inf and sum 0)
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) f[i] = m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[i] - M);
+        const float sum = wave_sum(f[0] * l[0] + f[1] * l[1]);
+        f4 o[K];
+#pragma unroll
+        for (uint32_t k = 0; k < K; ++k) o[k] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t q0 = 0;;) {
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t p = q0 + lane / L + u * G;
+                const float f0 = __shfl(f[0], p & 63), f1 = __shfl(f[1], p & 63), w = p >= parts ? 0.0f : p < 64 ? f0 : f1;
+#pragma unroll
+                for (uint32_t k = 0; k < K; ++k)
+                    if (w != 0.0f) o[k] += w * __builtin_bit_cast(f4, v[u][k]);  // (no infinity times a weight of 0)
+            }
+            if ((q0 += U * G) >= parts) break;
+            load(q0);
+        }
+#pragma unroll
+        for (uint32_t d = L; d < 64; d <<= 1)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) o[0][e] += __shfl_xor(o[0][e], d);
+        const uint32_t row = row0 + c;
         float* out = a.out + (size_t)(first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;
-        *reinterpret_cast<f4*>(out + x) = L == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o / L;
+        if (lane < L)
+#pragma unroll
+            for (uint32_t k = 0; k < K; ++k)
+                *reinterpret_cast<f4*>(out + (lane + L * k) * 4) = sum == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o[k] / sum;
     }
 }
 
@@ -567,6 +641,8 @@ template <int W, bool Q4>
 __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedAttn a, uint32_t units, uint32_t splits,
                                                                           uint32_t row_tiles, uint32_t chunk, bool join_apart) {
     constexpr int ST = W / 32, TV = W / 16, HALFROWS = 8;
+    // tiles of a wave on their way: two where their registers leave room for two waves per SIMD
+    constexpr int DEPTH = 1;
     using V = VHalf<W, Q4>;
     __shared__ __align__(16) uint8_t lds[W * 128];  // the queries' operands; at the end eight rows of each wave's sums
     __shared__ float wm[4][16], wl[4][16];
@@ -599,40 +675,44 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
             const uint32_t e = (tile_at(keys, min(i, max(keys.count, 1u) - 1)) * 32 + lane % 2 * 16) >> a.b.page_shift;
             held = e < a.b.table_stride ? table[e] : a.b.pages;
         };
-        KHalf<W, Q4> k[2];
-        V v[2];
-        bool ok[2] = {false, false};
-        auto bases = [&](uint32_t t, int half, size_t& off, uint32_t& slot) {
-            const uint32_t j = tile_at(keys, t) * 32 + half * 16;
-            uint32_t page = __builtin_amdgcn_readlane(held, (t - held_at) / 4 * 2 + half);
-            ok[half] = page < a.b.pages;
-            if (!ok[half]) page = 0;  // (some page: nothing of it is seen)
+        struct Stage {
+            KHalf<W, Q4> k[2];
+            V v[2];
+            bool ok[2];
+        } stage[DEPTH];
+        // (half i of tile t: its page's part, whether it has one, and its first slot)
+        auto base = [&](uint32_t t, int i, bool& ok, uint32_t& slot) {
+            const uint32_t j = tile_at(keys, t) * 32 + i * 16;
+            uint32_t page = __builtin_amdgcn_readlane(held, (t - held_at) / 4 * 2 + i);
+            ok = page < a.b.pages;
+            if (!ok) page = 0;  // (some page: nothing of it is seen)
             slot = j & (tokens - 1);
-            off = ((size_t)page * a.kv_heads + h) * part_bytes;
+            return ((size_t)page * a.kv_heads + h) * part_bytes;
         };
-        auto load_k = [&](uint32_t t) {
+        auto load_k = [&](uint32_t t, Stage& g) {
+            if (t >= held_at + 128) pages_from(t);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                size_t off;
                 uint32_t slot;
-                bases(t, i, off, slot);
-                k[i].load(a.k_pages + off, tokens, slot, lane);
+                const size_t off = base(t, i, g.ok[i], slot);
+                g.k[i].load(a.k_pages + off, tokens, slot, lane);
             }
         };
-        auto load_v = [&](uint32_t t) {
+        auto load_v = [&](uint32_t t, Stage& g) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                size_t off;
                 uint32_t slot;
-                bases(t, i, off, slot);
-                v[i].load(a.v_pages + off, tokens, slot, lane);
+                const size_t off = base(t, i, g.ok[i], slot);
+                g.v[i].load(a.v_pages + off, tokens, slot, lane);
             }
         };
-        if (t0 < t1) {
-            pages_from(t0);
-            load_k(t0);
-            load_v(t0);
-        }
+        if (t0 < t1) pages_from(t0);
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d)
+            if (t0 + 4 * d < t1) {
+                load_k(t0 + 4 * d, stage[d]);
+                load_v(t0 + 4 * d, stage[d]);
+            }
 
         // the queries as scaled fp16 pairs in operand order: thread (row tid / 16, lane of 16) takes octets of channels
         __syncthreads();  // (the last turn's sums are read)
@@ -687,10 +767,9 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
 #pragma unroll
         for (int t = 0; t < TV; ++t) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         Softmax sm;
-#pragma unroll 1
-        for (uint32_t t = t0; t < t1; t += 4) {
+        auto tile = [&](uint32_t t, Stage& here) {
             const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
-            const bool ok0 = ok[0], ok1 = ok[1], more = t + 4 < t1;
+            const bool ok0 = here.ok[0], ok1 = here.ok[1], more = t + 4 * DEPTH < t1;
             f4 sv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
             uint32_t qoff = lane * 16;
             asm volatile("" : "+v"(qoff));  // (the queries stay in LDS: hoisted into registers they make the others spill)
@@ -698,18 +777,14 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
             for (int st = 0; st < ST; ++st) {
                 if (st % 4 == 0) __builtin_amdgcn_sched_barrier(0);
                 const h8 hi = *reinterpret_cast<const h8*>(lds + st * 2048 + qoff), lo = *reinterpret_cast<const h8*>(lds + st * 2048 + 1024 + qoff);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const h8 A = k[i].operand(st);
-                    sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, lo, sv[i], 0, 0, 0);
-                    sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, hi, sv[i], 0, 0, 0);
-                }
+                const h8 A0 = here.k[0].operand(st), A1 = here.k[1].operand(st);
+                sv[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, lo, sv[0], 0, 0, 0);
+                sv[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, lo, sv[1], 0, 0, 0);
+                sv[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, hi, sv[0], 0, 0, 0);
+                sv[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, hi, sv[1], 0, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (more) {
-                if (t + 4 >= held_at + 128) pages_from(t + 4);
-                load_k(t + 4);
-            }
+            if (more) load_k(t + 4 * DEPTH, here);
             // a whole tile: every row sees every key
             const bool whole = ok0 & ok1 & (j0 + 31 <= hi_one) & ((j0 >= lo_one) | (j0 + 31 < first));
             if (!whole) {
@@ -721,7 +796,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                         const bool in = i ? ok1 : ok0;
                         sv[i][e] = in & (j <= hi_m) & ((j >= lo_m) | (j < first)) ? sv[i][e] : -INFINITY;
                         // keys that no row sees may be anything
-                        if (!(in & (j <= hi_all) & ((j >= lo_all) | (j < first)))) v[i].clear(e);
+                        if (!(in & (j <= hi_all) & ((j >= lo_all) | (j < first)))) here.v[i].clear(e);
                     }
             }
             h8 bh, bl;
@@ -734,16 +809,26 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
             for (int o = 0; o < TV / N; ++o) {
                 __builtin_amdgcn_sched_barrier(0);
                 uint32_t x[N][2], y[N][2];
-                v[0].template octet<N>(o, x);
-                v[1].template octet<N>(o, y);
+                here.v[0].template octet<N>(o, x);
+                here.v[1].template octet<N>(o, y);
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const h8 A = __builtin_bit_cast(h8, v4u{x[e][0], x[e][1], y[e][0], y[e][1]});
-                    acc[N * o + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[N * o + e], 0, 0, 0);
-                    acc[N * o + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[N * o + e], 0, 0, 0);
+                for (int e = 0; e < N; e += 2) {
+                    const h8 A0 = __builtin_bit_cast(h8, v4u{x[e][0], x[e][1], y[e][0], y[e][1]});
+                    const h8 A1 = __builtin_bit_cast(h8, v4u{x[e + 1][0], x[e + 1][1], y[e + 1][0], y[e + 1][1]});
+                    f4 &a0 = acc[N * o + e], &a1 = acc[N * o + e + 1];
+                    a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, bl, a0, 0, 0, 0);
+                    a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, bl, a1, 0, 0, 0);
+                    a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, bh, a0, 0, 0, 0);
+                    a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, bh, a1, 0, 0, 0);
                 }
             }
-            if (more) load_v(t + 4);
+            if (more) load_v(t + 4 * DEPTH, here);
+        };
+#pragma unroll 1
+        for (uint32_t t = t0; t < t1; t += 4 * DEPTH) {
+            tile(t, stage[0]);
+            if constexpr (DEPTH == 2)
+                if (t + 4 < t1) tile(t + 4, stage[1]);
         }
         const float lrun = row_total(sm.l);
 
@@ -832,24 +917,22 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
     }
 }
 
-// The sequence and row tile (of R rows) of a partial-sum slot.
-__device__ __forceinline__ uint32_t slot_sequence(const PagedAttn& a, uint32_t slot, uint32_t R, uint32_t& tile) {
-    const PagedBatch& b = a.b;
-    auto base = [&](uint32_t s) { return (uint32_t)((uint64_t)min(b.starts[s], b.tokens) * a.group / R) + s; };
-    const uint32_t seq = last_sequence(b.sequences, [&](uint32_t s) { return base(s) <= slot; });
-    tile = slot - min(slot, base(seq));
+// The sequence, its span and the row tile (of R rows) of a partial-sum slot.
+__device__ __forceinline__ uint32_t slot_sequence(const PagedAttn& a, uint32_t slot, uint32_t R, uint32_t& tile, Span& s) {
+    auto base = [&](uint32_t start, uint32_t k) { return (uint32_t)((uint64_t)min(start, a.b.tokens) * a.group / R) + k; };
+    const uint32_t seq = find_span(a.b, [&](uint32_t start, uint32_t k) { return base(start, k) <= slot; }, s, [] {});
+    tile = slot - min(slot, base(s.first, seq));
     return seq;
 }
 
-// Joins the chunks of (row tile, KV head) slots: a block per 1,024 sums of a slot, so that wide tiles of many chunks
-// are read by many CUs.
+// Joins the chunks of (row tile, KV head) slots, a block per four rows, so that wide tiles of many chunks are read by
+// many CUs.
 template <int W>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t splits, uint32_t chunk, uint32_t R) {
-    constexpr uint32_t C = 1024 / W < 1 ? 1 : 1024 / W;  // rows of a block
-    const uint32_t groups = R / C, slot = blockIdx.x / groups, c0 = blockIdx.x % groups * C, h = slot % a.kv_heads;
+    const uint32_t groups = R / 4, slot = blockIdx.x / groups, c0 = blockIdx.x % groups * 4, h = slot % a.kv_heads;
     uint32_t tile;
-    const uint32_t seq = slot_sequence(a, slot / a.kv_heads, R, tile);
-    const Span s = span_of(a.b.starts[seq], a.b.starts[seq + 1], a.b.lengths[seq], a.b);
+    Span s;
+    slot_sequence(a, slot / a.kv_heads, R, tile, s);
     const uint32_t rows = s.count * a.group;
     if (tile * R >= rows) return;
     const uint32_t nr = min(R, rows - tile * R);
@@ -859,7 +942,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
     uint32_t len, parts;
     chunks_of(keys.count, chunk, splits, len, parts);
     if (parts == 1) return;
-    join_parts<W>(a, a.part + (size_t)slot * splits * R * (W + 4), splits, parts, R, c0, min(nr, c0 + C), tile * R, s.first, h);
+    join_parts<W>(a, a.part + (size_t)slot * splits * R * (W + 4), splits, parts, R, c0, min(nr, c0 + 4), tile * R, s.first, h);
 }
 
 // ---- attention of many rows: prompts and further turns --------------------------------------------------
@@ -869,20 +952,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
 // one is on its way (in registers, then in the other buffer) and one barrier separates tiles.  Bound by the matrix
 // cores' 8 W multiply-adds per (row, key): both operands' pairs double the 4 W of the product.
 //
-// K lies in LDS as the first product reads it, piece ((half, step), lane) of 16 bytes; V transposed and its channels
-// ordered by their place in an octet (E values of a load), so that writes (lanes along octets and keys) and reads
-// (lanes along a tile's 16 rows) both sweep LDS in address order.  Q4 blocks become fp16 on the way.
+// K lies in LDS as the first product reads it, piece ((half, step), lane) of 16 bytes; V transposed, piece (tile of 16
+// channels, lane), its channels ordered by their place in an octet (E values of a load), so that both what a wave
+// reads and what it writes are consecutive.  4-bit blocks become fp16 on the way.
 
-// The order of a product's instructions: its LDS operands are requested kAhead reads before the two products that take
-// one (left to itself the compiler requests each where it is needed, and every product waits for LDS).
-constexpr int kAhead = 4;
+// The order of a product's instructions: its LDS operands are requested two pairs before the four products that take
+// a pair (left to itself the compiler requests each where it is needed, and every product waits for LDS).  N: pairs.
 template <int N>
 __device__ __forceinline__ void pipeline_operands() {
-    __builtin_amdgcn_sched_group_barrier(0x100, N < kAhead ? N : kAhead, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, N < 2 ? 2 : 4, 0);
 #pragma unroll
     for (int f = 0; f < N; ++f) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-        if (f + kAhead < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        if (f + 2 < N) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
 }
 
@@ -908,8 +990,8 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
     slot = slots - 1 - slot;  // (a sequence's last rows, which see the most keys, first)
     const uint32_t h = hs % a.kv_heads, split = hs / a.kv_heads;
     uint32_t rt;
-    const uint32_t seq = slot_sequence(a, slot, R, rt);
-    const Span s = span_of(a.b.starts[seq], a.b.starts[seq + 1], a.b.lengths[seq], a.b);
+    Span s;
+    const uint32_t seq = slot_sequence(a, slot, R, rt, s);
     const uint32_t rows = s.count * a.group, tokens = 1u << a.b.page_shift;
     if (rt * R >= rows) return;
     const uint32_t nr = min((uint32_t)R, rows - rt * R);
@@ -932,14 +1014,19 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
         held = e < a.b.table_stride ? table[e] : a.b.pages;
     };
     // The next tile's K and V on their way.  Thread: pieces of K tid + 256 i, in LDS order (octets: half, step, lane; 4-bit
-    // blocks: half, block, row); of V: half, octet of channels, four keys 4 u .. 4 u + 3.  Where a half's share is whole
-    // waves (UK, UV), its address is scalar plus a constant per lane.
+    // blocks: half, block, row), their addresses scalar plus a constant per lane where a half's share is whole waves
+    // (UK); of V: four keys 4 u .. 4 u + 3 of a half, octet o of channels, so that 32 lanes write 256 bytes of LDS in a row.
     constexpr uint32_t PK = Q4 ? W : W * 4;  // pieces of K
-    constexpr bool UK = PK / 2 >= 64, UV = W / 2 >= 64;
+    constexpr bool UK = PK / 2 >= 64;
     v4u kr[NK];
     uint32_t kd[Q4 ? NK : 1];
     uint32_t vr[NV][4][Q4 ? 1 : 4], vd[Q4 ? NV : 1][4];
-    auto half_of = [&](bool uniform, uint32_t i, uint32_t of) { return ((uniform ? wave * 64 : tid) + 256 * i) / of; };
+    auto v_piece = [](uint32_t e, uint32_t& half, uint32_t& u, uint32_t& o) {
+        constexpr uint32_t O = W / 8 < 16 ? W / 8 : 16;
+        half = e / O % 2;
+        u = e / (2 * O) % 4;
+        o = e / (8 * O) * O + e % O;
+    };
     auto load = [&](uint32_t t) {
         if (t >= held_at + 32) pages_from(t);
         const uint32_t j0 = tile_at(keys, t) * 32;
@@ -954,7 +1041,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
         }
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
-            const uint32_t half = half_of(UK, i, PK / 2), e = (tid + 256 * i) % (PK / 2);
+            const uint32_t half = ((UK ? wave * 64 : tid) + 256 * i) / (PK / 2), e = (tid + 256 * i) % (PK / 2);
             const uint8_t* p = a.k_pages + (half ? off[1] : off[0]);
             const uint32_t sl = half ? slot_[1] : slot_[0];
             if constexpr (!Q4) {
@@ -971,7 +1058,8 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (W < 256 && tid >= W) break;
-            const uint32_t half = half_of(UV, i, W / 2), e = (tid + 256 * i) % (W / 2), u = e % 4, o = e / 4;
+            uint32_t half, u, o;
+            v_piece(tid + 256 * i, half, u, o);
             const uint8_t* p = a.v_pages + (half ? off[1] : off[0]);
             const uint32_t sl = half ? slot_[1] : slot_[0];
 #pragma unroll
@@ -1011,10 +1099,11 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
         if (!(p0 & p1 & (j0 + 31 <= hi_all) & ((j0 >= lo_all) | (j0 + 31 < first))))  // keys that no row sees may be anything
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const uint32_t e = (tid + 256 * i) % (W / 2), half = (tid + 256 * i) / (W / 2);
+                uint32_t half, u, o;
+                v_piece(tid + 256 * i, half, u, o);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int32_t key = j0 + (int32_t)(half * 16 + e % 4 * 4) + j;
+                    const int32_t key = j0 + (int32_t)(half * 16 + u * 4) + j;
                     if (!((half ? p1 : p0) & (key <= hi_all) & ((key >= lo_all) | (key < first)))) {
 #pragma unroll
                         for (int r = 0; r < (Q4 ? 1 : 4); ++r) vr[i][j][r] = 0;
@@ -1025,7 +1114,8 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (W < 256 && tid >= W) break;
-            const uint32_t half = (tid + 256 * i) / (W / 2), e = (tid + 256 * i) % (W / 2), u = e % 4, o = e / 4;
+            uint32_t half, u, o;
+            v_piece(tid + 256 * i, half, u, o);
             uint32_t x[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1039,12 +1129,13 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
                     for (int r = 0; r < 4; ++r) x[j][r] = __builtin_bit_cast(uint32_t, y[r]);
                 }
             }
-            // channel 8 o + d: row (d % E) W / E + (8 o + d) / E of the transposed tile; its eight-key piece u, half `half`
-            uint8_t* dst = vl + (o * (8 / E) * 64 + u * 16 + half * 8);
+            // channel 8 o + d: row r = (d % E) W / E + (8 o + d) / E of the transposed tile; its eight-key piece u, half `half`
+            const uint32_t r = o * (8 / E);
+            uint8_t* dst = vl + (r / 16 * 1024 + r % 16 * 16 + u * 256 + half * 8);
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
                 const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
-                *reinterpret_cast<u2*>(dst + ((d % E) * (W / E) + d / E) * 64) =
+                *reinterpret_cast<u2*>(dst + (d % E) * (W / E) * 64 + d / E * 16) =
                     u2{__builtin_amdgcn_perm(x[1][d / 2], x[0][d / 2], sel), __builtin_amdgcn_perm(x[3][d / 2], x[2][d / 2], sel)};
             }
         }
@@ -1115,13 +1206,15 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
         if (!idle & (j0 <= hi_any) & ((j0 + 31 >= lo_any) | (j0 < first))) {
             f4 sv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-            for (int f = 0; f < 2 * ST; ++f) {
-                const int i = f & 1, st = f >> 1;
-                const h8 A = *reinterpret_cast<const h8*>(kl + ((i * ST + st) * 64 + lane) * 16);
-                sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, ql[st], sv[i], 0, 0, 0);
-                sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, qh[st], sv[i], 0, 0, 0);
+            for (int st = 0; st < ST; ++st) {
+                const h8 A0 = *reinterpret_cast<const h8*>(kl + (st * 64 + lane) * 16);
+                const h8 A1 = *reinterpret_cast<const h8*>(kl + ((ST + st) * 64 + lane) * 16);
+                sv[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, ql[st], sv[0], 0, 0, 0);
+                sv[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, ql[st], sv[1], 0, 0, 0);
+                sv[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, qh[st], sv[0], 0, 0, 0);
+                sv[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, qh[st], sv[1], 0, 0, 0);
             }
-            pipeline_operands<2 * ST>();
+            pipeline_operands<ST>();
             const bool whole = (page_ok & 3) == 3 && j0 + 31 <= hi_one && (j0 >= lo_one || j0 + 31 < first);
             if (!whole)
 #pragma unroll
@@ -1137,12 +1230,15 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
                 for (int v = 0; v < TV; ++v) acc[v] *= f;
             });
 #pragma unroll
-            for (int v = 0; v < TV; ++v) {
-                const h8 A = *reinterpret_cast<const h8*>(vl + ((16 * v + m) * 4 + g) * 16);
-                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[v], 0, 0, 0);
-                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[v], 0, 0, 0);
+            for (int v = 0; v < TV; v += 2) {
+                const h8 A0 = *reinterpret_cast<const h8*>(vl + (v * 64 + lane) * 16);
+                const h8 A1 = *reinterpret_cast<const h8*>(vl + (v * 64 + 64 + lane) * 16);
+                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, bl, acc[v], 0, 0, 0);
+                acc[v + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, bl, acc[v + 1], 0, 0, 0);
+                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, bh, acc[v], 0, 0, 0);
+                acc[v + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, bh, acc[v + 1], 0, 0, 0);
             }
-            pipeline_operands<TV>();
+            pipeline_operands<TV / 2>();
         }
         if (t + 1 < t1) {
             store(t + 1, lds[(t + 1 - t0) & 1][0], lds[(t + 1 - t0) & 1][1]);
@@ -1214,10 +1310,18 @@ static hipError_t by_layout(uint32_t width, bool q4, F f) {
 }
 
 hipError_t launch_kv_append(const KvAppend& a, uint32_t width, bool q4, hipStream_t s) {
-    const uint32_t groups = (a.q_heads + 2 * a.kv_heads + 3) / 4, tasks = a.b.tokens * groups;
+    // four rows a wave where they still fill the chip: 256 CUs of 32 waves
+    const uint32_t heads = a.q_heads + 2 * a.kv_heads;
+    const bool four = (uint64_t)a.b.tokens * heads >= 4 * 8192;
+    const uint32_t per = four ? 16 : 4, groups = (heads + per - 1) / per, tasks = a.b.tokens * groups;
     return by_layout(width, q4, [&](auto w, auto t) {
-        hipLaunchKernelGGL((kv_append_kernel<decltype(w)::value, decltype(t)::value>), dim3(min(tasks, 1u << 20)), dim3(256), 0,
-                           s, a, groups, tasks);
+        constexpr int W = decltype(w)::value;
+        constexpr bool Q4 = decltype(t)::value;
+        const dim3 grid(min(tasks, 1u << 20)), block(256);
+        if (four)
+            hipLaunchKernelGGL((kv_append_kernel<W, Q4, 4>), grid, block, 0, s, a, groups, tasks);
+        else
+            hipLaunchKernelGGL((kv_append_kernel<W, Q4, 1>), grid, block, 0, s, a, groups, tasks);
         return hipGetLastError();
     });
 }
@@ -1243,8 +1347,7 @@ hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, c
         }
         hipError_t e = hipGetLastError();
         if (e == hipSuccess && p.join_apart) {
-            constexpr uint32_t C = 1024 / W < 1 ? 1 : 1024 / W;
-            hipLaunchKernelGGL(paged_join_kernel<W>, dim3(p.slots * a.kv_heads * (p.rows / C)), block, 0, s, a, p.splits, p.chunk, p.rows);
+            hipLaunchKernelGGL(paged_join_kernel<W>, dim3(p.slots * a.kv_heads * (p.rows / 4)), block, 0, s, a, p.splits, p.chunk, p.rows);
             e = hipGetLastError();
         }
         return e;

@@ -29,103 +29,141 @@ __device__ __forceinline__ uint64_t wave_best(uint64_t k) {
     return k;
 }
 
-template <bool VEC>
+// Q: quads of a thread (a slice is 1,024 Q tokens); VEC: rows of logits and out are 16-byte aligned.
+template <int Q, bool VEC>
 __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
-    extern __shared__ uint32_t named[];  // per token of the slice: history count | (bias index + 1) << 16
+    constexpr uint32_t SLICE = 1024 * Q;
+    __shared__ __align__(16) uint32_t named[SLICE];  // per token of the slice: history count | (bias index + 1) << 16
     __shared__ uint64_t best[4];
     __shared__ uint32_t worst[4], last;
     const uint32_t row = blockIdx.x / a.slices, part = blockIdx.x % a.slices, tid = threadIdx.x;
-    const uint32_t base = part * a.slice, n = min(a.slice, a.vocabulary - base);
-    for (uint32_t i = tid; i < a.slice; i += 256) named[i] = 0;
-    __syncthreads();
+    const uint32_t base = part * SLICE, n = min(SLICE, a.vocabulary - base);
+    // the slice is on its way while its history is counted: thread's quad q at tokens 1024 q + 4 tid
+    const float* x = a.logits + (size_t)row * a.stride + base;
+    float v[Q][4];
+    uint32_t bits[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const uint32_t i = 1024 * q + 4 * tid;
+        if (VEC && i + 4 <= n) {
+            const float4 f = *reinterpret_cast<const float4*>(x + i);
+            v[q][0] = f.x, v[q][1] = f.y, v[q][2] = f.z, v[q][3] = f.w;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) v[q][e] = i + e < n ? x[i + e] : -INFINITY;
+        }
+        bits[q] = a.mask && i < n ? a.mask[(size_t)row * a.mask_stride + (base + i) / 32] : 0xFFFFFFFFu;
+    }
+    // and so are the row's lists: their first entries whether they count or not
+    const bool past = a.penalties && a.history;
+    const uint32_t* h = a.history + (size_t)row * a.history_stride;
+    const uint32_t* ids = a.bias_ids + (size_t)row * a.bias_stride;
+    constexpr int H = 4, B = 2;
+    uint32_t hist[H], bias[B];
+#pragma unroll
+    for (int u = 0; u < H; ++u) hist[u] = past && tid + 256 * u < a.history_stride ? h[tid + 256 * u] : 0;
+#pragma unroll
+    for (int u = 0; u < B; ++u) bias[u] = a.bias_ids && tid + 256 * u < a.bias_stride ? ids[tid + 256 * u] : 0;
+    const uint32_t hist_len = past ? min(a.history_len[row], a.history_stride) : 0;
+    const uint32_t bias_len = a.bias_ids ? min(a.bias_len[row], a.bias_stride) : 0;
     double rep = 1.0, pres = 0.0, freq = 0.0;
-    if (a.penalties && a.history) {
+    if (past) {
         rep = a.penalties[3 * row];
         pres = a.penalties[3 * row + 1];
         freq = a.penalties[3 * row + 2];
-        const uint32_t len = min(a.history_len[row], a.history_stride);
-        const uint32_t* h = a.history + (size_t)row * a.history_stride;
-        for (uint32_t i = tid; i < len; i += 256) {
-            const uint32_t t = h[i] - base;
-            if (t < n) atomicAdd(&named[t], 1u);
-        }
     }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) *reinterpret_cast<uint4*>(named + 1024 * q + 4 * tid) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    const float* bv = nullptr;
-    if (a.bias_ids) {
+    if (hist_len) {
+        auto count = [&](uint32_t id, uint32_t i) {
+            if (i < hist_len && id - base < n) atomicAdd(&named[id - base], 1u);
+        };
+#pragma unroll
+        for (int u = 0; u < H; ++u) count(hist[u], tid + 256 * u);
+        for (uint32_t i0 = tid + 256 * H; i0 < hist_len; i0 += 1024) {
+            uint32_t t[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) t[u] = i0 + 256 * u < hist_len ? h[i0 + 256 * u] : 0;
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) count(t[u], i0 + 256 * u);
+        }
+        __syncthreads();
+    }
+    const float* bv = a.bias_values + (size_t)row * a.bias_stride;
+    if (bias_len) {
         // an id's last bias counts: the largest index (the count below it is the same for all of the id's)
-        const uint32_t len = min(a.bias_len[row], a.bias_stride);
-        const uint32_t* ids = a.bias_ids + (size_t)row * a.bias_stride;
-        bv = a.bias_values + (size_t)row * a.bias_stride;
-        for (uint32_t i = tid; i < len; i += 256) {
-            const uint32_t t = ids[i] - base;
-            if (t < n) atomicMax(&named[t], (i + 1) << 16 | (named[t] & 0xFFFFu));
-        }
+        auto note = [&](uint32_t id, uint32_t i) {
+            if (i < bias_len && id - base < n) atomicMax(&named[id - base], (i + 1) << 16 | (named[id - base] & 0xFFFFu));
+        };
+#pragma unroll
+        for (int u = 0; u < B; ++u) note(bias[u], tid + 256 * u);
+        for (uint32_t i = tid + 256 * B; i < bias_len; i += 256) note(ids[i], i);
+        __syncthreads();
     }
-    __syncthreads();
-    const float* x = a.logits + (size_t)row * a.stride + base;
-    float* y = a.out ? a.out + (size_t)row * a.out_stride + base : nullptr;
-    const uint32_t* mask = a.mask ? a.mask + (size_t)row * a.mask_stride : nullptr;
-    uint64_t top = 0;
-    uint32_t bad = 0;
-    auto one = [&](float v, uint32_t i, uint32_t allow) {
-        const uint32_t w = named[i];
-        if (w) {
-            double d = v;
-            if (w & 0xFFFFu) d = (d > 0.0 ? d / rep : d * rep) - __dadd_rn(__dmul_rn(freq, (double)(w & 0xFFFFu)), pres);
-            if (w >> 16) d += (double)bv[(w >> 16) - 1];
-            v = (float)d;
-        }
-        if (!allow) v = -INFINITY;
-        const uint64_t key = (uint64_t)order_of(v) << 32 | (uint32_t)~(base + i);
-        top = key > top ? key : top;
-        bad |= !(v < INFINITY);
-        return v;
-    };
-    if constexpr (VEC) {
-        for (uint32_t i = 4 * tid; i < n; i += 1024) {
-            float v[4];
-            const bool whole = i + 4 <= n;
-            if (whole) {
-                const float4 f = *reinterpret_cast<const float4*>(x + i);
-                v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-            } else {
-                for (uint32_t e = 0; e < 4; ++e) v[e] = i + e < n ? x[i + e] : -INFINITY;
-            }
-            const uint32_t bits = mask ? mask[(base + i) / 32] >> ((base + i) % 32) : 0xFu;
+    float high = -INFINITY;  // of the thread's, its lowest token (they come in rising order)
+    uint32_t at = 0;
+    bool odd = false;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const uint32_t i = 1024 * q + 4 * tid;
+        const uint4 w4 = *reinterpret_cast<const uint4*>(named + i);
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        if (w4.x | w4.y | w4.z | w4.w)
+#pragma unroll
             for (uint32_t e = 0; e < 4; ++e)
-                if (i + e < n) v[e] = one(v[e], i + e, bits >> e & 1);
-            if (y) {
-                if (whole)
-                    *reinterpret_cast<float4*>(y + i) = make_float4(v[0], v[1], v[2], v[3]);
-                else
-                    for (uint32_t e = 0; e < 4; ++e)
-                        if (i + e < n) y[i + e] = v[e];
+                if (w[e]) {
+                    double d = v[q][e];
+                    const double c = w[e] & 0xFFFFu;
+                    if (w[e] & 0xFFFFu) d = (d > 0.0 ? d / rep : d * rep) - __dadd_rn(__dmul_rn(freq, c), pres);
+                    if (w[e] >> 16) d += (double)bv[(w[e] >> 16) - 1];
+                    v[q][e] = (float)d;
+                }
+        const uint32_t allow = bits[q] >> ((base + i) % 32);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            if (!(allow >> e & 1)) v[q][e] = -INFINITY;
+            if (v[q][e] > high) {
+                high = v[q][e];
+                at = i + e;
             }
-        }
-    } else {
-        for (uint32_t i = tid; i < n; i += 256) {
-            const float v = one(x[i], i, mask ? mask[(base + i) / 32] >> ((base + i) % 32) & 1 : 1u);
-            if (y) y[i] = v;
+            odd |= !(v[q][e] < INFINITY);
         }
     }
-    top = wave_best(top);
-    const uint64_t any = __ballot(bad);
+    uint64_t top = wave_best((uint64_t)order_of(high) << 32 | (uint32_t)~(base + at));
+    uint32_t bad;
+    const uint64_t any = __ballot(odd);
     if ((tid & 63) == 0) {
         best[tid >> 6] = top;
         worst[tid >> 6] = any != 0;
     }
     __syncthreads();
-    // the slices of a row meet at its ticket; the last one in takes the largest of their keys
+    // The slices of a row meet at its ticket; the last one in takes the largest of their keys.  The ticket is drawn
+    // before the slice is stored, which it need not wait for.
     const __amdgpu_buffer_rsrc_t prs =
         __builtin_amdgcn_make_buffer_rsrc(a.part + (size_t)row * a.slices, 0, (int)(a.slices * 16), 0x00020000);
+    uint32_t ticket = 0;
     if (tid == 0) {
         for (int w = 1; w < 4; ++w) top = best[w] > top ? best[w] : top;
         bad = worst[0] | worst[1] | worst[2] | worst[3];
         __builtin_amdgcn_raw_buffer_store_b128(v4u{(uint32_t)(top >> 32), (uint32_t)top, bad, 0u}, prs, part * 16, 0, kPartSC1);
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
-        last = __hip_atomic_fetch_add(a.tickets + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.slices - 1;
+        ticket = __hip_atomic_fetch_add(a.tickets + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    if (a.out) {
+        float* y = a.out + (size_t)row * a.out_stride + base;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const uint32_t i = 1024 * q + 4 * tid;
+            if (VEC && i + 4 <= n)
+                *reinterpret_cast<float4*>(y + i) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
+            else
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (i + e < n) y[i + e] = v[q][e];
+        }
+    }
+    if (tid == 0) last = ticket == a.slices - 1;
     __syncthreads();
     if (!last || tid >= 64) return;
     top = 0;
@@ -149,8 +187,11 @@ __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
 
 hipError_t launch_logits_select(const LogitsSelect& a, hipStream_t s) {
     const bool vec = ((uintptr_t)a.logits | (uintptr_t)a.out) % 16 == 0 && a.stride % 4 == 0 && (!a.out || a.out_stride % 4 == 0);
-    hipLaunchKernelGGL(vec ? logits_select_kernel<true> : logits_select_kernel<false>, dim3(a.rows * a.slices), dim3(256),
-                       a.slice * 4, s, a);
+    const dim3 grid(a.rows * a.slices), block(256);
+    if (a.slice == 4096)
+        hipLaunchKernelGGL((vec ? logits_select_kernel<4, true> : logits_select_kernel<4, false>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((vec ? logits_select_kernel<1, true> : logits_select_kernel<1, false>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 

@@ -307,6 +307,7 @@ int af_logits_select_workspace(const af_logits_args* p, size_t* bytes) {
     if (!p || !bytes) return fail(AF_ERR_INVALID, "null argument");
     if (p->rows == 0 || p->rows > AF_MAX_LOGIT_ROWS || p->vocabulary == 0 || p->vocabulary > 0x1000000u)
         return fail(AF_ERR_INVALID, "invalid number of rows or tokens of the vocabulary");
+    if ((uint64_t)p->rows * p->vocabulary > 1ull << 34) return fail(AF_ERR_INVALID, "rows times vocabulary above 2^34");
     const uint32_t slice = logits_slice(p->rows, p->vocabulary);
     *bytes = kTicketBytes + (size_t)p->rows * ((p->vocabulary + slice - 1) / slice) * 16;
     return AF_OK;
