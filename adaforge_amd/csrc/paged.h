@@ -83,6 +83,14 @@ AF_HD uint32_t page_part_bytes(bool q4, uint32_t page, uint32_t width) {
 constexpr uint32_t kTickets = 16384;
 constexpr size_t kTicketBytes = kTickets * 4;
 
+// The distance of `count` tickets: up to a cache line of 128 bytes.  The memory side takes the draws of one line in
+// turn, about 5 ns each: 4,096 blocks that drew from 64 adjacent words took 20 us for it.
+inline uint32_t ticket_stride(uint64_t count) {
+    uint32_t s = 32;
+    while (s > 1 && count * s > kTickets) s /= 2;
+    return s;
+}
+
 // What the split of an attention call depends on: sizes, and the caller's hints.
 struct AttnShape {
     uint32_t sequences, tokens, kv_heads, group, width, window, sinks;
@@ -122,7 +130,7 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     const uint64_t pairs = (uint64_t)a.sequences * a.kv_heads;  // (at most 2^22: checked by the call)
     const uint32_t tiles = longest_tiles(a, tokens);
     p.row_tiles = (uint32_t)(((uint64_t)tokens * a.group + 15) / 16);
-    p.rows = p.row_tiles > 2 ? kManyRows : 16;
+    p.rows = p.row_tiles > 4 ? kManyRows : 16;
     p.slots = row_slots(a, p.rows);
     if (p.row_tiles * pairs > 1u << 22) p.row_tiles = most(1, (uint32_t)((1u << 22) / pairs));
     const uint64_t sums = (uint64_t)p.slots * a.kv_heads;
@@ -135,7 +143,7 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
         splits = sums > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / sums)));
     } else {
         p.units = (uint32_t)sums;
-        splits = most(least(most(1, 256 / p.units), most(1, tiles / 8)), least(most(1, 1024 / p.units), most(1, tiles / 16)));
+        splits = most(least(most(1, 512 / p.units), most(1, tiles / 8)), least(most(1, 1024 / p.units), most(1, tiles / 16)));
         splits = least(splits, 16);
     }
     p.chunk = (tiles + splits - 1) / splits;
@@ -175,6 +183,7 @@ struct PagedAttn {
     float scale;
     PagedBatch b;
     uint32_t* tickets;
+    uint32_t ticket_stride;
     float* part;
 };
 hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, const AttnPlan& plan, hipStream_t s);
@@ -194,16 +203,15 @@ struct LogitsSelect {
     uint32_t mask_stride;
     uint32_t* result;
     uint32_t* tickets;
-    uint4* part;  // one (key high, key low, bad, 0) per slice of a row
-    uint32_t slice, slices;
+    uint32_t ticket_stride;
+    uint4* part;      // one (key high, key low, bad, 0) per slice of a row
+    uint32_t slices;
 };
 hipError_t launch_logits_select(const LogitsSelect& a, hipStream_t s);
 
 #endif
 
-// The choice of a token: a block takes a slice of a row: 4,096 tokens where that makes 1,024 blocks and more, else 1,024.
-AF_HD uint32_t logits_slice(uint32_t rows, uint32_t vocabulary) {
-    return (uint64_t)rows * vocabulary >= (uint64_t)4096 * 1024 ? 4096 : 1024;
-}
+// Tokens of a row that a block takes in the choice of a token.
+constexpr uint32_t kLogitsSlice = 4096;
 
 }  // namespace af

@@ -77,19 +77,17 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 // the low bits of 0x6400 is the fp16 number 1024 + n, four bits higher 1024 + 16 n, so n - 8 is one exact operation,
 // and d (n - 8) one rounding.
 __device__ __forceinline__ void unpack4(uint32_t w, _Float16 d, h2 (&o)[4]) {
-    // (one instruction each; from w & mask | magic the compiler makes two)
-    auto code = [](uint32_t v, uint32_t mask) {
-        uint32_t r;
-        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(v), "s"(mask), "v"(0x64006400u));
-        return __builtin_bit_cast(h2, r);
-    };
+    // (in registers that the compiler does not know, mask and magic make one instruction; as constants two)
+    uint32_t even = 0x000F000Fu, odd = 0x00F000F0u, magic = 0x64006400u;
+    asm("" : "+s"(even), "+s"(odd), "+v"(magic));
+    auto code = [&](uint32_t v, uint32_t mask) { return __builtin_bit_cast(h2, (v & mask) | magic); };
     const h2 low = {(_Float16)-1032.0f, (_Float16)-1032.0f}, high = {(_Float16)-72.0f, (_Float16)-72.0f};
     const h2 part = {(_Float16)0.0625f, (_Float16)0.0625f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const uint32_t v = w >> (8 * i);
-        o[2 * i] = (code(v, 0x000F000Fu) + low) * h2{d, d};
-        o[2 * i + 1] = __builtin_elementwise_fma(code(v, 0x00F000F0u), part, high) * h2{d, d};
+        o[2 * i] = (code(v, even) + low) * h2{d, d};
+        o[2 * i + 1] = __builtin_elementwise_fma(code(v, odd), part, high) * h2{d, d};
     }
 }
 
@@ -411,6 +409,35 @@ __device__ __forceinline__ void operand_of(uint32_t o, uint32_t& step, uint32_t&
     }
 }
 
+// Where 32 tiles' halves (16 keys, in one page) lie: lane l holds that of half l % 2 of tile first + l / 2 step, so that
+// the table is read, and an offset computed, once in 32 tiles; a tile's base addresses are then lane reads.
+template <int W, bool Q4>
+struct HalfTable {
+    uint32_t lo, hi;  // byte offset of the half's first row (of codes) in the pages
+    uint32_t scales;  // 4 bits: from there to its first row of scales
+    uint64_t ok;      // lanes whose half has a page (others: some page, nothing of which is seen)
+    uint32_t first;
+
+    __device__ __forceinline__ void fill(const PagedAttn& a, const Tiles& keys, uint32_t seq, uint32_t h, uint32_t t, uint32_t step,
+                                         uint32_t end) {
+        const uint32_t lane = threadIdx.x & 63, tokens = 1u << a.b.page_shift;
+        const uint32_t j = tile_at(keys, min(t + lane / 2 * step, end - 1)) * 32 + lane % 2 * 16, e = j >> a.b.page_shift;
+        const uint32_t page = e < a.b.table_stride ? a.b.table[(size_t)seq * a.b.table_stride + e] : a.b.pages;
+        const uint32_t slot = j & (tokens - 1);
+        const uint64_t off = ((uint64_t)(page < a.b.pages ? page : 0) * a.kv_heads + h) * page_part_bytes(Q4, tokens, W) +
+                             slot * (Q4 ? W / 2 : W * 2);
+        ok = __ballot(page < a.b.pages);
+        lo = (uint32_t)off;
+        hi = (uint32_t)(off >> 32);
+        scales = tokens * (W / 2) + slot * (W / 16) - slot * (W / 2);
+        first = t;
+    }
+    __device__ __forceinline__ uint64_t offset(uint32_t l) const {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, l) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, l);
+    }
+    __device__ __forceinline__ uint32_t scales_at(uint32_t l) const { return Q4 ? __builtin_amdgcn_readlane(scales, l) : 0; }
+};
+
 // Rows of K of one half tile (16 keys): a lane's loads, and its operand of a step.
 template <int W, bool Q4>
 struct KHalf {
@@ -418,16 +445,16 @@ struct KHalf {
     v4u c[Q4 ? (W >= 128 ? W / 128 : 1) : 1];
     uint32_t d[Q4 ? (W >= 128 ? W / 128 : 1) : 1];  // (fp16 scales)
 
-    // part: the page's part, tokens: of a page, slot: of the half's first key
-    __device__ __forceinline__ void load(const uint8_t* part, uint32_t tokens, uint32_t slot, uint32_t lane) {
+    // rows: of the half (4 bits: codes), scales: from there to its scales
+    __device__ __forceinline__ void load(const uint8_t* rows, uint32_t scales, uint32_t lane) {
         const uint32_t m = lane & 15, g = lane >> 4;
         if constexpr (!Q4) {
-            const auto* p = gp(part + (size_t)slot * (W * 2)) + (m * (W * 2) + g * 16);
+            const auto* p = gp(rows) + (m * (W * 2) + g * 16);
 #pragma unroll
             for (int s = 0; s < W / 32; ++s) f[s] = *(const __attribute__((address_space(1))) v4u*)(p + 64 * s);
         } else {
-            const auto* sc = gp(part + (size_t)tokens * (W / 2) + slot * (W / 16));
-            const auto* p = gp(part + (size_t)slot * (W / 2));
+            const auto* sc = gp(rows + scales);
+            const auto* p = gp(rows);
             if constexpr (W >= 128) {
 #pragma unroll
                 for (int i = 0; i < W / 128; ++i) {
@@ -460,12 +487,12 @@ struct VHalf {
     uint32_t w[4][C][R];
     uint32_t d[Q4 ? 4 : 1];  // (fp16 scales)
 
-    __device__ __forceinline__ void load(const uint8_t* part, uint32_t tokens, uint32_t slot, uint32_t lane) {
+    __device__ __forceinline__ void load(const uint8_t* rows, uint32_t scales, uint32_t lane) {
         const uint32_t m = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (!Q4) {
-                const auto* p = gp(part + (size_t)slot * (W * 2)) + (g * (W * 8) + m * (2 * E) + j * (W * 2));
+                const auto* p = gp(rows) + (g * (W * 8) + m * (2 * E) + j * (W * 2));
 #pragma unroll
                 for (int c = 0; c < C; ++c)
                     if constexpr (E == 8) {
@@ -476,7 +503,7 @@ struct VHalf {
                         w[j][c][0] = x.x, w[j][c][1] = x.y;
                     }
             } else {
-                const auto* p = gp(part + (size_t)slot * (W / 2)) + (g * (W * 2) + m * (W / 32) + j * (W / 2));
+                const auto* p = gp(rows) + (g * (W * 2) + m * (W / 32) + j * (W / 2));
                 if constexpr (W == 512) {
                     const v4u x = *(const __attribute__((address_space(1))) v4u*)(p);
                     w[j][0][0] = x.x, w[j][0][1] = x.y, w[j][0][2] = x.z, w[j][0][3] = x.w;
@@ -486,11 +513,10 @@ struct VHalf {
                 } else if constexpr (W == 128) {
                     w[j][0][0] = *(const __attribute__((address_space(1))) uint32_t*)(p);
                 } else {  // four of a word's eight: pairs 0 and 1, or 2 and 3
-                    const auto* q = gp(part + (size_t)slot * (W / 2)) + (g * (W * 2) + m / 2 * 4 + j * (W / 2));
+                    const auto* q = gp(rows) + (g * (W * 2) + m / 2 * 4 + j * (W / 2));
                     w[j][0][0] = *(const __attribute__((address_space(1))) uint32_t*)(q) >> (m % 2 * 8);
                 }
-                d[j] = *(const __attribute__((address_space(1))) uint16_t*)(gp(part + (size_t)tokens * (W / 2) + slot * (W / 16)) +
-                                                                            (g * (W / 4) + m * W / 512 * 2 + j * (W / 16)));
+                d[j] = *(const __attribute__((address_space(1))) uint16_t*)(gp(rows + scales) + (g * (W / 4) + m * W / 512 * 2 + j * (W / 16)));
             }
         }
     }
@@ -531,10 +557,10 @@ struct VHalf {
 struct Softmax {
     float m = -INFINITY, l = 0.0f, off = 0.0f;  // l: the sum over this lane's keys; off = kProbBits - m
 
-    // Weights of the lane's eight keys, scores s (-inf: not seen) times qs, as fp16 pairs; scale(f) takes the factor of
-    // the sums so far where it is not 1 (lanes of a column agree).
+    // Takes in the lane's scores of eight keys (times qs; -inf: not seen): scale(f) gets the factor of the sums so far
+    // where it is not 1 (lanes of a column agree).
     template <typename F>
-    __device__ __forceinline__ void step(const f4 (&s)[2], float qs, h8& hi, h8& lo, F scale) {
+    __device__ __forceinline__ void rise(const f4 (&s)[2], float qs, F scale) {
         const float mine = qs * fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         if (__ballot(mine > m + kRise)) {
@@ -545,23 +571,29 @@ struct Softmax {
             l *= al;
             scale(al);
         }
-        uint32_t ph[4], pl[4];
-        float sum[2];
+    }
+
+    // Their weights, as fp16 pairs, in eight slices: 0 .. 3 two weights each, 4 .. 7 a pair's halves.
+    struct Weights {
+        float p[8];
+        uint32_t hi[4], lo[4];
+        __device__ __forceinline__ h8 high() const { return __builtin_bit_cast(h8, v4u{hi[0], hi[1], hi[2], hi[3]}); }
+        __device__ __forceinline__ h8 low() const { return __builtin_bit_cast(h8, v4u{lo[0], lo[1], lo[2], lo[3]}); }
+    };
+    __device__ __forceinline__ void slice(int k, const f4 (&s)[2], float qs, Weights& w) {
+        if (k < 4) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], qs, off));
-            sum[i] = (p[0] + p[1]) + (p[2] + p[3]);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                ph[2 * i + e] = pack_f16(p[2 * e], p[2 * e + 1]);
-                pl[2 * i + e] = pack_f16(less_half<0>(p[2 * e], ph[2 * i + e]), less_half<1>(p[2 * e + 1], ph[2 * i + e]));
-            }
+            for (int e = 0; e < 2; ++e) w.p[2 * k + e] = __builtin_amdgcn_exp2f(fmaf(s[k / 2][k % 2 * 2 + e], qs, off));
+        } else {
+            k -= 4;
+            w.hi[k] = pack_f16(w.p[2 * k], w.p[2 * k + 1]);
+            w.lo[k] = pack_f16(less_half<0>(w.p[2 * k], w.hi[k]), less_half<1>(w.p[2 * k + 1], w.hi[k]));
+            if (k == 3) l += ((w.p[0] + w.p[1]) + (w.p[2] + w.p[3])) + ((w.p[4] + w.p[5]) + (w.p[6] + w.p[7]));
         }
-        l += sum[0] + sum[1];
-        hi = __builtin_bit_cast(h8, v4u{ph[0], ph[1], ph[2], ph[3]});
-        lo = __builtin_bit_cast(h8, v4u{pl[0], pl[1], pl[2], pl[3]});
+    }
+    __device__ __forceinline__ void weights(const f4 (&s)[2], float qs, Weights& w) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) slice(k, s, qs, w);
     }
 };
 
@@ -641,8 +673,6 @@ template <int W, bool Q4>
 __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedAttn a, uint32_t units, uint32_t splits,
                                                                           uint32_t row_tiles, uint32_t chunk, bool join_apart) {
     constexpr int ST = W / 32, TV = W / 16, HALFROWS = 8;
-    // tiles of a wave on their way: two where their registers leave room for two waves per SIMD
-    constexpr int DEPTH = 1;
     using V = VHalf<W, Q4>;
     __shared__ __align__(16) uint8_t lds[W * 128];  // the queries' operands; at the end eight rows of each wave's sums
     __shared__ float wm[4][16], wl[4][16];
@@ -652,9 +682,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
     const uint32_t h = unit % a.kv_heads, seq = unit / a.kv_heads % a.b.sequences, tile0 = unit / a.kv_heads / a.b.sequences;
     const uint32_t start = a.b.starts[seq];
     const Span s = span_of(start, a.b.starts[seq + 1], a.b.lengths[seq], a.b);
-    const uint32_t rows = s.count * a.group, tokens = 1u << a.b.page_shift;
-    const uint32_t part_bytes = page_part_bytes(Q4, tokens, W);
-    const uint32_t* table = a.b.table + (size_t)seq * a.b.table_stride;
+    const uint32_t rows = s.count * a.group;
 
     // (one turn unless a sequence has more rows than the launch was told)
     for (uint32_t rt = tile0; rt * 16 < rows; rt += row_tiles) {
@@ -667,52 +695,31 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         if (split >= parts) continue;
         const uint32_t t0 = split * len + wave, t1 = min((split + 1) * len, keys.count);
 
-        // the pages of this wave's halves of tiles: lane l holds that of half l % 2 of its tile l / 2, 32 tiles at a time
-        uint32_t held = 0, held_at = t0;
-        auto pages_from = [&](uint32_t t) {
-            held_at = t;
-            const uint32_t i = t + lane / 2 * 4;
-            const uint32_t e = (tile_at(keys, min(i, max(keys.count, 1u) - 1)) * 32 + lane % 2 * 16) >> a.b.page_shift;
-            held = e < a.b.table_stride ? table[e] : a.b.pages;
-        };
+        HalfTable<W, Q4> where;  // of this wave's tiles
         struct Stage {
             KHalf<W, Q4> k[2];
             V v[2];
             bool ok[2];
-        } stage[DEPTH];
-        // (half i of tile t: its page's part, whether it has one, and its first slot)
-        auto base = [&](uint32_t t, int i, bool& ok, uint32_t& slot) {
-            const uint32_t j = tile_at(keys, t) * 32 + i * 16;
-            uint32_t page = __builtin_amdgcn_readlane(held, (t - held_at) / 4 * 2 + i);
-            ok = page < a.b.pages;
-            if (!ok) page = 0;  // (some page: nothing of it is seen)
-            slot = j & (tokens - 1);
-            return ((size_t)page * a.kv_heads + h) * part_bytes;
-        };
+        } here;
         auto load_k = [&](uint32_t t, Stage& g) {
-            if (t >= held_at + 128) pages_from(t);
+            if (t >= where.first + 128) where.fill(a, keys, seq, h, t, 4, keys.count);
+            const uint32_t l = (t - where.first) / 2;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                uint32_t slot;
-                const size_t off = base(t, i, g.ok[i], slot);
-                g.k[i].load(a.k_pages + off, tokens, slot, lane);
+                g.ok[i] = where.ok >> (l + i) & 1;
+                g.k[i].load(a.k_pages + where.offset(l + i), where.scales_at(l + i), lane);
             }
         };
         auto load_v = [&](uint32_t t, Stage& g) {
+            const uint32_t l = (t - where.first) / 2;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t slot;
-                const size_t off = base(t, i, g.ok[i], slot);
-                g.v[i].load(a.v_pages + off, tokens, slot, lane);
-            }
+            for (int i = 0; i < 2; ++i) g.v[i].load(a.v_pages + where.offset(l + i), where.scales_at(l + i), lane);
         };
-        if (t0 < t1) pages_from(t0);
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d)
-            if (t0 + 4 * d < t1) {
-                load_k(t0 + 4 * d, stage[d]);
-                load_v(t0 + 4 * d, stage[d]);
-            }
+        if (t0 < t1) {
+            where.fill(a, keys, seq, h, t0, 4, keys.count);
+            load_k(t0, here);
+            load_v(t0, here);
+        }
 
         // the queries as scaled fp16 pairs in operand order: thread (row tid / 16, lane of 16) takes octets of channels
         __syncthreads();  // (the last turn's sums are read)
@@ -767,9 +774,10 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
 #pragma unroll
         for (int t = 0; t < TV; ++t) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         Softmax sm;
-        auto tile = [&](uint32_t t, Stage& here) {
+#pragma unroll 1
+        for (uint32_t t = t0; t < t1; t += 4) {
             const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
-            const bool ok0 = here.ok[0], ok1 = here.ok[1], more = t + 4 * DEPTH < t1;
+            const bool ok0 = here.ok[0], ok1 = here.ok[1], more = t + 4 < t1;
             f4 sv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
             uint32_t qoff = lane * 16;
             asm volatile("" : "+v"(qoff));  // (the queries stay in LDS: hoisted into registers they make the others spill)
@@ -777,14 +785,15 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
             for (int st = 0; st < ST; ++st) {
                 if (st % 4 == 0) __builtin_amdgcn_sched_barrier(0);
                 const h8 hi = *reinterpret_cast<const h8*>(lds + st * 2048 + qoff), lo = *reinterpret_cast<const h8*>(lds + st * 2048 + 1024 + qoff);
-                const h8 A0 = here.k[0].operand(st), A1 = here.k[1].operand(st);
-                sv[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, lo, sv[0], 0, 0, 0);
-                sv[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, lo, sv[1], 0, 0, 0);
-                sv[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, hi, sv[0], 0, 0, 0);
-                sv[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, hi, sv[1], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const h8 A = here.k[i].operand(st);
+                    sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, lo, sv[i], 0, 0, 0);
+                    sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, hi, sv[i], 0, 0, 0);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (more) load_k(t + 4 * DEPTH, here);
+            if (more) load_k(t + 4, here);
             // a whole tile: every row sees every key
             const bool whole = ok0 & ok1 & (j0 + 31 <= hi_one) & ((j0 >= lo_one) | (j0 + 31 < first));
             if (!whole) {
@@ -799,11 +808,13 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                         if (!(in & (j <= hi_all) & ((j >= lo_all) | (j < first)))) here.v[i].clear(e);
                     }
             }
-            h8 bh, bl;
-            sm.step(sv, qs, bh, bl, [&](float f) {
+            sm.rise(sv, qs, [&](float f) {
 #pragma unroll
                 for (int i = 0; i < TV; ++i) acc[i] *= f;
             });
+            Softmax::Weights w;
+            sm.weights(sv, qs, w);
+            const h8 bh = w.high(), bl = w.low();
             constexpr int N = TV < 8 ? TV : 8;
 #pragma unroll
             for (int o = 0; o < TV / N; ++o) {
@@ -812,23 +823,14 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                 here.v[0].template octet<N>(o, x);
                 here.v[1].template octet<N>(o, y);
 #pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    const h8 A0 = __builtin_bit_cast(h8, v4u{x[e][0], x[e][1], y[e][0], y[e][1]});
-                    const h8 A1 = __builtin_bit_cast(h8, v4u{x[e + 1][0], x[e + 1][1], y[e + 1][0], y[e + 1][1]});
-                    f4 &a0 = acc[N * o + e], &a1 = acc[N * o + e + 1];
-                    a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, bl, a0, 0, 0, 0);
-                    a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, bl, a1, 0, 0, 0);
-                    a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, bh, a0, 0, 0, 0);
-                    a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, bh, a1, 0, 0, 0);
+                for (int e = 0; e < N; ++e) {
+                    const h8 A = __builtin_bit_cast(h8, v4u{x[e][0], x[e][1], y[e][0], y[e][1]});
+                    f4& to = acc[N * o + e];
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, to, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, to, 0, 0, 0);
                 }
             }
-            if (more) load_v(t + 4 * DEPTH, here);
-        };
-#pragma unroll 1
-        for (uint32_t t = t0; t < t1; t += 4 * DEPTH) {
-            tile(t, stage[0]);
-            if constexpr (DEPTH == 2)
-                if (t + 4 < t1) tile(t + 4, stage[1]);
+            if (more) load_v(t + 4, here);
         }
         const float lrun = row_total(sm.l);
 
@@ -909,10 +911,10 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
         __syncthreads();
         if (tid == 0)
-            last = __hip_atomic_fetch_add(a.tickets + slot, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+            last = __hip_atomic_fetch_add(a.tickets + slot * a.ticket_stride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
         __syncthreads();
         if (!last) continue;
-        if (tid == 0) __hip_atomic_store(a.tickets + slot, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) __hip_atomic_store(a.tickets + slot * a.ticket_stride, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         join_parts<W>(a, a.part + (size_t)slot * splits * 16 * (W + 4), splits, parts, 16, 0, nr, rt * 16, s.first, h);
     }
 }
@@ -956,20 +958,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
 // channels, lane), its channels ordered by their place in an octet (E values of a load), so that both what a wave
 // reads and what it writes are consecutive.  4-bit blocks become fp16 on the way.
 
-// The order of a product's instructions: its LDS operands are requested two pairs before the four products that take
-// a pair (left to itself the compiler requests each where it is needed, and every product waits for LDS).  N: pairs.
-template <int N>
-__device__ __forceinline__ void pipeline_operands() {
-    __builtin_amdgcn_sched_group_barrier(0x100, N < 2 ? 2 : 4, 0);
-#pragma unroll
-    for (int f = 0; f < N; ++f) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-        if (f + 2 < N) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    }
-}
-
 template <int W, bool Q4>
-__global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(PagedAttn a, uint32_t slots, uint32_t splits,
+__global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_many_kernel(PagedAttn a, uint32_t slots, uint32_t splits,
                                                                                 uint32_t chunk) {
     constexpr int ST = W / 32, TV = W / 16, R = kManyRows;
     constexpr int E = W / 16 < 8 ? W / 16 : 8;  // channels of an octet
@@ -992,7 +982,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
     uint32_t rt;
     Span s;
     const uint32_t seq = slot_sequence(a, slot, R, rt, s);
-    const uint32_t rows = s.count * a.group, tokens = 1u << a.b.page_shift;
+    const uint32_t rows = s.count * a.group;
     if (rt * R >= rows) return;
     const uint32_t nr = min((uint32_t)R, rows - rt * R);
     const int32_t plo = s.pos0 + (int32_t)(rt * R / a.group), phi = s.pos0 + (int32_t)((rt * R + nr - 1) / a.group);
@@ -1001,17 +991,23 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
     chunks_of(keys.count, chunk, splits, len, parts);
     if (split >= parts) return;
     const uint32_t t0 = split * len, t1 = min(t0 + len, keys.count);
-    const uint32_t part_bytes = page_part_bytes(Q4, tokens, W);
-    const uint32_t* table = a.b.table + (size_t)seq * a.b.table_stride;
     const int32_t edge = (int32_t)s.end - 1, first = (int32_t)min(a.sinks, 1u << 30);
     const int32_t hi_all = min(phi, edge), lo_all = first_seen(plo, a.window);
 
-    // page numbers: lane l holds that of half l % 2 of tile held_at + l / 2
-    uint32_t held = 0, held_at = t0;
-    auto pages_from = [&](uint32_t t) {
-        held_at = t;
-        const uint32_t e = (tile_at(keys, min(t + lane / 2, keys.count - 1)) * 32 + lane % 2 * 16) >> a.b.page_shift;
-        held = e < a.b.table_stride ? table[e] : a.b.pages;
+    HalfTable<W, Q4> where;
+    // where a tile's halves lie (the last tile again past the end), and whether they have a page
+    struct Ref {
+        uint64_t off0, off1;
+        uint32_t scales0, scales1;
+        int32_t j0;
+        uint32_t ok;  // bits 0 and 1
+    };
+    auto ref = [&](uint32_t t) {
+        t = min(t, t1 - 1);
+        if (t >= where.first + 32) where.fill(a, keys, seq, h, t, 1, t1);
+        const uint32_t l = (t - where.first) * 2;
+        return Ref{where.offset(l), where.offset(l + 1), where.scales_at(l), where.scales_at(l + 1), (int32_t)tile_at(keys, t) * 32,
+                   (uint32_t)(where.ok >> l) & 3};
     };
     // The next tile's K and V on their way.  Thread: pieces of K tid + 256 i, in LDS order (octets: half, step, lane; 4-bit
     // blocks: half, block, row), their addresses scalar plus a constant per lane where a half's share is whole waves
@@ -1027,122 +1023,113 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
         u = e / (2 * O) % 4;
         o = e / (8 * O) * O + e % O;
     };
-    auto load = [&](uint32_t t) {
-        if (t >= held_at + 32) pages_from(t);
-        const uint32_t j0 = tile_at(keys, t) * 32;
-        size_t off[2];
-        uint32_t slot_[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint32_t page = __builtin_amdgcn_readlane(held, (t - held_at) * 2 + i);
-            if (page >= a.b.pages) page = 0;  // (some page: nothing of it is seen)
-            slot_[i] = (j0 + 16 * i) & (tokens - 1);
-            off[i] = ((size_t)page * a.kv_heads + h) * part_bytes;
-        }
+    auto load_k = [&](const Ref& r) {
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
             const uint32_t half = ((UK ? wave * 64 : tid) + 256 * i) / (PK / 2), e = (tid + 256 * i) % (PK / 2);
-            const uint8_t* p = a.k_pages + (half ? off[1] : off[0]);
-            const uint32_t sl = half ? slot_[1] : slot_[0];
+            const uint8_t* p = a.k_pages + (r.off0 + (half ? r.off1 - r.off0 : 0));
             if constexpr (!Q4) {
                 const uint32_t st = UK ? (wave * 64 + 256 * i) % (PK / 2) / 64 : e / 64;
-                const auto* q = gp(p + (size_t)sl * (W * 2) + st * 64) + (m * (W * 2) + g * 16);
+                const auto* q = gp(p) + (st * 64 + m * (W * 2) + g * 16);
                 kr[i] = *(const __attribute__((address_space(1))) v4u*)q;
             } else if (PK >= 256 || tid < PK) {
-                const auto* q = gp(p + (size_t)sl * (W / 2)) + (e % 16 * (W / 2) + e / 16 * 16);
-                const auto* d = gp(p + (size_t)tokens * (W / 2) + sl * (W / 16)) + (e % 16 * (W / 16) + e / 16 * 2);
+                const auto* q = gp(p) + (e % 16 * (W / 2) + e / 16 * 16);
+                const auto* d = gp(p + (r.scales0 + (half ? r.scales1 - r.scales0 : 0))) + (e % 16 * (W / 16) + e / 16 * 2);
                 kr[i] = *(const __attribute__((address_space(1))) v4u*)q;
                 kd[i] = *(const __attribute__((address_space(1))) uint16_t*)d;
             }
         }
+    };
+    auto load_v = [&](const Ref& r) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (W < 256 && tid >= W) break;
             uint32_t half, u, o;
             v_piece(tid + 256 * i, half, u, o);
-            const uint8_t* p = a.v_pages + (half ? off[1] : off[0]);
-            const uint32_t sl = half ? slot_[1] : slot_[0];
+            const uint8_t* p = a.v_pages + (r.off0 + (half ? r.off1 - r.off0 : 0));
+            const uint32_t scales = r.scales0 + (half ? r.scales1 - r.scales0 : 0);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if constexpr (!Q4) {
-                    const auto* q = gp(p + (size_t)sl * (W * 2)) + (u * (W * 8) + o * 16 + j * (W * 2));
+                    const auto* q = gp(p) + (u * (W * 8) + o * 16 + j * (W * 2));
                     const v4u x = *(const __attribute__((address_space(1))) v4u*)q;
                     vr[i][j][0] = x.x, vr[i][j][1] = x.y, vr[i][j][2] = x.z, vr[i][j][3] = x.w;
                 } else {
-                    const auto* q = gp(p + (size_t)sl * (W / 2)) + (u * (W * 2) + o * 4 + j * (W / 2));
-                    const auto* d = gp(p + (size_t)tokens * (W / 2) + sl * (W / 16)) + (u * (W / 4) + o / 4 * 2 + j * (W / 16));
+                    const auto* q = gp(p) + (u * (W * 2) + o * 4 + j * (W / 2));
+                    const auto* d = gp(p + scales) + (u * (W / 4) + o / 4 * 2 + j * (W / 16));
                     vr[i][j][0] = *(const __attribute__((address_space(1))) uint32_t*)q;
                     vd[i][j] = *(const __attribute__((address_space(1))) uint16_t*)d;
                 }
         }
     };
-    auto store = [&](uint32_t t, uint8_t* kl, uint8_t* vl) {
-        const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const uint32_t e = tid + 256 * i;
-            if constexpr (!Q4) {
-                *reinterpret_cast<v4u*>(kl + e * 16) = kr[i];
-            } else if (PK >= 256 || tid < PK) {
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    h2 x[4];
-                    unpack4(kr[i][w], __builtin_bit_cast(_Float16, (uint16_t)kd[i]), x);
-                    *reinterpret_cast<v4u*>(kl + (e / 16 * 64 + w * 16 + e % 16) * 16) =
-                        v4u{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1]),
-                            __builtin_bit_cast(uint32_t, x[2]), __builtin_bit_cast(uint32_t, x[3])};
-                }
-            }
+    // the tile into LDS, in slices: KS of K (one write each), then VS of V (4-bit: a key's octet unpacked; then a channel
+    // of four keys written)
+    constexpr int KS = Q4 ? 4 * NK : NK, VU = Q4 ? 4 : 0, VS = NV * (VU + 8);
+    auto store_k = [&](int k, uint8_t* kl) {
+        if constexpr (!Q4) {
+            *reinterpret_cast<v4u*>(kl + (tid + 256 * k) * 16) = kr[k];
+        } else if (PK >= 256 || tid < PK) {
+            const uint32_t e = tid + 256 * (k / 4);
+            h2 x[4];
+            unpack4(kr[k / 4][k % 4], __builtin_bit_cast(_Float16, (uint16_t)kd[k / 4]), x);
+            *reinterpret_cast<v4u*>(kl + (e / 16 * 64 + k % 4 * 16 + e % 16) * 16) =
+                v4u{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1]),
+                    __builtin_bit_cast(uint32_t, x[2]), __builtin_bit_cast(uint32_t, x[3])};
         }
-        const bool p0 = __builtin_amdgcn_readlane(held, (t - held_at) * 2) < a.b.pages;
-        const bool p1 = __builtin_amdgcn_readlane(held, (t - held_at) * 2 + 1) < a.b.pages;
-        if (!(p0 & p1 & (j0 + 31 <= hi_all) & ((j0 >= lo_all) | (j0 + 31 < first))))  // keys that no row sees may be anything
+    };
+    // values of keys that no row sees may be anything
+    auto clear_v = [&](const Ref& r) {
+        if (!((r.ok == 3) & (r.j0 + 31 <= hi_all) & ((r.j0 >= lo_all) | (r.j0 + 31 < first))))
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 uint32_t half, u, o;
                 v_piece(tid + 256 * i, half, u, o);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int32_t key = j0 + (int32_t)(half * 16 + u * 4) + j;
-                    if (!((half ? p1 : p0) & (key <= hi_all) & ((key >= lo_all) | (key < first)))) {
+                    const int32_t key = r.j0 + (int32_t)(half * 16 + u * 4) + j;
+                    if (!((r.ok >> half & 1) & (key <= hi_all) & ((key >= lo_all) | (key < first)))) {
 #pragma unroll
-                        for (int r = 0; r < (Q4 ? 1 : 4); ++r) vr[i][j][r] = 0;
+                        for (int x = 0; x < (Q4 ? 1 : 4); ++x) vr[i][j][x] = 0;
                         if constexpr (Q4) vd[i][j] = 0;
                     }
                 }
             }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (W < 256 && tid >= W) break;
-            uint32_t half, u, o;
-            v_piece(tid + 256 * i, half, u, o);
-            uint32_t x[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (!Q4) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[j][r] = vr[i][j][r];
-                } else {
-                    h2 y[4];
-                    unpack4(vr[i][j][0], __builtin_bit_cast(_Float16, (uint16_t)vd[i][j]), y);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[j][r] = __builtin_bit_cast(uint32_t, y[r]);
-                }
-            }
-            // channel 8 o + d: row r = (d % E) W / E + (8 o + d) / E of the transposed tile; its eight-key piece u, half `half`
-            const uint32_t r = o * (8 / E);
-            uint8_t* dst = vl + (r / 16 * 1024 + r % 16 * 16 + u * 256 + half * 8);
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
-                *reinterpret_cast<u2*>(dst + (d % E) * (W / E) * 64 + d / E * 16) =
-                    u2{__builtin_amdgcn_perm(x[1][d / 2], x[0][d / 2], sel), __builtin_amdgcn_perm(x[3][d / 2], x[2][d / 2], sel)};
-            }
-        }
     };
+    uint32_t vx[4][4];
+    auto store_v = [&](int k, uint8_t* vl) {
+        if (W < 256 && tid >= W) return;
+        const int i = k / (VU + 8);
+        k %= VU + 8;
+        if (k < VU) {
+            h2 y[4];
+            unpack4(vr[i][k][0], __builtin_bit_cast(_Float16, (uint16_t)vd[i][k]), y);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) vx[k][r] = __builtin_bit_cast(uint32_t, y[r]);
+            return;
+        }
+        // channel 8 o + d: row r = (d % E) W / E + (8 o + d) / E of the transposed tile; its eight-key piece u, half `half`
+        const int d = k - VU;
+        uint32_t half, u, o;
+        v_piece(tid + 256 * i, half, u, o);
+        const uint32_t r = o * (8 / E), sel = d & 1 ? 0x07060302u : 0x05040100u;
+        uint32_t x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = Q4 ? vx[j][d / 2] : vr[i][j][Q4 ? 0 : d / 2];
+        *reinterpret_cast<u2*>(vl + (r / 16 * 1024 + r % 16 * 16 + u * 256 + half * 8) + (d % E) * (W / E) * 64 + d / E * 16) =
+            u2{__builtin_amdgcn_perm(x[1], x[0], sel), __builtin_amdgcn_perm(x[3], x[2], sel)};
+    };
+    auto store = [&](int k, uint8_t* kl, uint8_t* vl) {
+        if (k < KS)
+            store_k(k, kl);
+        else
+            store_v(k - KS, vl);
+    };
+    Ref now, next, after;
     if (t0 < t1) {
-        pages_from(t0);
-        load(t0);
+        where.fill(a, keys, seq, h, t0, 1, t1);
+        now = ref(t0);
+        load_k(now);
+        load_v(now);
     }
 
     // the queries: lane (column m, g) holds channels 32 s + 8 g .. + 7 of step s, as scaled fp16 pairs
@@ -1176,76 +1163,161 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_many_kernel(Paged
                 }
             }
     }
-    // this wave's rows: what any and what every one of them sees
     const bool idle = row0 >= rows;
     const int32_t wlo = s.pos0 + (int32_t)(min(row0, rows - 1) / a.group);
     const int32_t whi = s.pos0 + (int32_t)(min(row0 + 15, rows - 1) / a.group);
-    const int32_t hi_any = min(whi, edge), lo_any = first_seen(wlo, a.window), hi_one = min(wlo, edge), lo_one = first_seen(whi, a.window);
+    const int32_t hi_one = min(wlo, edge), lo_one = first_seen(whi, a.window);  // (what every one of its rows sees)
     const int32_t hi_m = min(pos, edge), lo_m = first_seen(pos, a.window);
 
     f4 acc[TV];
     Softmax sm;
 #pragma unroll
     for (int t = 0; t < TV; ++t) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t page_ok = 0;  // whether the halves of the tile in use, and of the next, have a page (bits 0, 1 and 2, 3)
-    auto oks = [&](uint32_t t) {
-        return (uint32_t)(__builtin_amdgcn_readlane(held, (t - held_at) * 2) < a.b.pages) |
-               (uint32_t)(__builtin_amdgcn_readlane(held, (t - held_at) * 2 + 1) < a.b.pages) << 1;
-    };
-    if (t0 < t1) {
-        store(t0, lds[0][0], lds[0][1]);
-        page_ok = oks(t0);
-        if (t0 + 1 < t1) load(t0 + 1);
-    }
-    __syncthreads();
-#pragma unroll 1
-    for (uint32_t t = t0; t < t1; ++t) {
-        const uint8_t *kl = lds[(t - t0) & 1][0], *vl = lds[(t - t0) & 1][1];
-        const int32_t j0 = (int32_t)tile_at(keys, t) * 32;
-        // (a tile that none of the wave's rows sees, as at the causal edge, is passed over)
-        if (!idle & (j0 <= hi_any) & ((j0 + 31 >= lo_any) | (j0 < first))) {
-            f4 sv[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    // S^T of a tile, from its K in LDS; piece(k) does the k-th of eight slices of other work meanwhile
+    constexpr int AHEAD = W == 512 ? 3 : 2;  // operands requested ahead of their two products
+    auto scores = [&](const uint8_t* kl, f4 (&sv)[2], auto piece) {
+        auto at = [&](int f) { return *reinterpret_cast<const h8*>(kl + ((f % 2 * ST + f / 2) * 64 + lane) * 16); };
+        sv[0] = sv[1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        h8 A[2 * ST];
 #pragma unroll
-            for (int st = 0; st < ST; ++st) {
-                const h8 A0 = *reinterpret_cast<const h8*>(kl + (st * 64 + lane) * 16);
-                const h8 A1 = *reinterpret_cast<const h8*>(kl + ((ST + st) * 64 + lane) * 16);
-                sv[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, ql[st], sv[0], 0, 0, 0);
-                sv[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, ql[st], sv[1], 0, 0, 0);
-                sv[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, qh[st], sv[0], 0, 0, 0);
-                sv[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, qh[st], sv[1], 0, 0, 0);
-            }
-            pipeline_operands<ST>();
-            const bool whole = (page_ok & 3) == 3 && j0 + 31 <= hi_one && (j0 >= lo_one || j0 + 31 < first);
-            if (!whole)
+        for (int f = 0; f < AHEAD; ++f) A[f] = at(f);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+        for (int f = 0; f < 2 * ST; ++f) {
+            if (f + AHEAD < 2 * ST) A[f + AHEAD] = at(f + AHEAD);
+            sv[f % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[f], ql[f / 2], sv[f % 2], 0, 0, 0);
+            sv[f % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[f], qh[f / 2], sv[f % 2], 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int32_t j = j0 + 16 * i + 4 * (int32_t)g + e;
-                        sv[i][e] = (page_ok >> i & 1) & (j <= hi_m) & ((j >= lo_m) | (j < first)) ? sv[i][e] : -INFINITY;
-                    }
-            h8 bh, bl;
-            sm.step(sv, qs, bh, bl, [&](float f) {
-#pragma unroll
-                for (int v = 0; v < TV; ++v) acc[v] *= f;
-            });
-#pragma unroll
-            for (int v = 0; v < TV; v += 2) {
-                const h8 A0 = *reinterpret_cast<const h8*>(vl + (v * 64 + lane) * 16);
-                const h8 A1 = *reinterpret_cast<const h8*>(vl + (v * 64 + 64 + lane) * 16);
-                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, bl, acc[v], 0, 0, 0);
-                acc[v + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, bl, acc[v + 1], 0, 0, 0);
-                acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A0, bh, acc[v], 0, 0, 0);
-                acc[v + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A1, bh, acc[v + 1], 0, 0, 0);
-            }
-            pipeline_operands<TV / 2>();
+            for (int k = 0; k < 8; ++k)
+                if (k * ST / 4 == f) piece(k);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (t + 1 < t1) {
-            store(t + 1, lds[(t + 1 - t0) & 1][0], lds[(t + 1 - t0) & 1][1]);
-            page_ok = oks(t + 1);
-            if (t + 2 < t1) load(t + 2);
+    };
+    f4 sv[2];
+    // the scores of tile `now`: masked where not every row sees every key, and taken into the running maximum
+    auto enter = [&] {
+        if (!((now.ok == 3) & (now.j0 + 31 <= hi_one) & ((now.j0 >= lo_one) | (now.j0 + 31 < first))))
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int32_t j = now.j0 + 16 * i + 4 * (int32_t)g + e;
+                    sv[i][e] = (now.ok >> i & 1) & (j <= hi_m) & ((j >= lo_m) | (j < first)) ? sv[i][e] : -INFINITY;
+                }
+        sm.rise(sv, qs, [&](float f) {
+#pragma unroll
+            for (int v = 0; v < TV; ++v) acc[v] *= f;
+        });
+    };
+    if constexpr (W >= 256) {
+        // K is one tile ahead of V: while tile t's weights are taken, tile t + 1's scores are computed, and while V of t is
+        // multiplied, K of t + 2 and V of t + 1 go to LDS.  The order of the instructions is the source's, a few at a time:
+        // LDS operands requested AHEAD, other work behind each operand's two products (left to itself the compiler
+        // requests each operand where it is needed and keeps the products apart from the rest).
+        if (t0 < t1) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) store_k(k, lds[0][0]);
+            clear_v(now);
+#pragma unroll
+            for (int k = 0; k < VS; ++k) store_v(k, lds[0][1]);
+            next = ref(t0 + 1);
+            load_k(next);
+            load_v(next);
+            __syncthreads();
+            scores(lds[0][0], sv, [](int) {});
+#pragma unroll
+            for (int k = 0; k < KS; ++k) store_k(k, lds[1][0]);
+            after = ref(t0 + 2);
+            load_k(after);
         }
         __syncthreads();
+#pragma unroll 1
+        for (uint32_t t = t0, b = 0; t < t1; ++t, b ^= 1) {
+            Softmax::Weights w;
+            f4 ahead[2];
+            if (!idle) {
+                enter();
+                __builtin_amdgcn_sched_barrier(0);
+                scores(lds[b ^ 1][0], ahead, [&](int k) { sm.slice(k, sv, qs, w); });
+            }
+            clear_v(next);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!idle) {
+                const h8 bh = w.high(), bl = w.low();
+                const uint8_t* vl = lds[b][1];
+                auto at = [&](int v) { return *reinterpret_cast<const h8*>(vl + (v * 64 + lane) * 16); };
+                h8 A[TV];
+#pragma unroll
+                for (int v = 0; v < AHEAD; ++v) A[v] = at(v);
+#pragma unroll
+                for (int v = 0; v < TV; ++v) {
+                    if (v + AHEAD < TV) A[v + AHEAD] = at(v + AHEAD);
+                    acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[v], bl, acc[v], 0, 0, 0);
+                    acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[v], bh, acc[v], 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < KS + VS; ++k)
+                        if (k * TV / (KS + VS) == v) store(k, lds[b][0], lds[b ^ 1][1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                sv[0] = ahead[0];
+                sv[1] = ahead[1];
+            } else {
+#pragma unroll
+                for (int k = 0; k < KS + VS; ++k) store(k, lds[b][0], lds[b ^ 1][1]);
+            }
+            load_v(after);
+            now = next;
+            next = after;
+            after = ref(t + 3);
+            load_k(after);
+            __syncthreads();
+        }
+    } else {
+        // (narrow heads: few products a tile; more waves per SIMD overlap them better than one wave's own order)
+        if (t0 < t1) {
+#pragma unroll
+            for (int k = 0; k < KS + VS; ++k) {
+                if (k == KS) clear_v(now);
+                store(k, lds[0][0], lds[0][1]);
+            }
+            next = ref(t0 + 1);
+            load_k(next);
+            load_v(next);
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (uint32_t t = t0, b = 0; t < t1; ++t, b ^= 1) {
+            if (!idle) {
+                const uint8_t *kl = lds[b][0] + lane * 16, *vl = lds[b][1] + lane * 16;
+                sv[0] = sv[1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int f = 0; f < 2 * ST; ++f) {
+                    const int i = f & 1, st = f >> 1;
+                    const h8 A = *reinterpret_cast<const h8*>(kl + (i * ST + st) * 1024);
+                    sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, ql[st], sv[i], 0, 0, 0);
+                    sv[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, qh[st], sv[i], 0, 0, 0);
+                }
+                enter();
+                Softmax::Weights w;
+                sm.weights(sv, qs, w);
+                const h8 bh = w.high(), bl = w.low();
+#pragma unroll
+                for (int v = 0; v < TV; ++v) {
+                    const h8 A = *reinterpret_cast<const h8*>(vl + v * 1024);
+                    acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[v], 0, 0, 0);
+                    acc[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[v], 0, 0, 0);
+                }
+            }
+            if (t + 1 < t1) {
+                clear_v(next);
+#pragma unroll
+                for (int k = 0; k < KS + VS; ++k) store(k, lds[b ^ 1][0], lds[b ^ 1][1]);
+                now = next;
+                next = ref(t + 2);
+                load_k(next);
+                load_v(next);
+            }
+            __syncthreads();
+        }
     }
     if (idle) return;
 

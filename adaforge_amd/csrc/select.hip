@@ -29,22 +29,23 @@ __device__ __forceinline__ uint64_t wave_best(uint64_t k) {
     return k;
 }
 
-// Q: quads of a thread (a slice is 1,024 Q tokens); VEC: rows of logits and out are 16-byte aligned.
-template <int Q, bool VEC>
-__global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
-    constexpr uint32_t SLICE = 1024 * Q;
+// T: threads, which take the slice's tokens by quads; VEC: rows of logits and out are 16-byte aligned.
+template <int T, bool VEC>
+__global__ __launch_bounds__(T) void logits_select_kernel(LogitsSelect a) {
+    constexpr uint32_t SLICE = kLogitsSlice;
+    constexpr int Q = SLICE / 4 / T, WAVES = T / 64;  // quads of a thread
     __shared__ __align__(16) uint32_t named[SLICE];  // per token of the slice: history count | (bias index + 1) << 16
-    __shared__ uint64_t best[4];
-    __shared__ uint32_t worst[4], last;
+    __shared__ uint64_t best[WAVES];
+    __shared__ uint32_t worst[WAVES], last;
     const uint32_t row = blockIdx.x / a.slices, part = blockIdx.x % a.slices, tid = threadIdx.x;
     const uint32_t base = part * SLICE, n = min(SLICE, a.vocabulary - base);
-    // the slice is on its way while its history is counted: thread's quad q at tokens 1024 q + 4 tid
+    // the slice is on its way while its history is counted: thread's quad q at tokens 4 (T q + tid)
     const float* x = a.logits + (size_t)row * a.stride + base;
     float v[Q][4];
     uint32_t bits[Q];
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-        const uint32_t i = 1024 * q + 4 * tid;
+        const uint32_t i = 4 * (T * q + tid);
         if (VEC && i + 4 <= n) {
             const float4 f = *reinterpret_cast<const float4*>(x + i);
             v[q][0] = f.x, v[q][1] = f.y, v[q][2] = f.z, v[q][3] = f.w;
@@ -58,12 +59,12 @@ __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
     const bool past = a.penalties && a.history;
     const uint32_t* h = a.history + (size_t)row * a.history_stride;
     const uint32_t* ids = a.bias_ids + (size_t)row * a.bias_stride;
-    constexpr int H = 4, B = 2;
+    constexpr int H = 1024 / T, B = T < 512 ? 512 / T : 1;
     uint32_t hist[H], bias[B];
 #pragma unroll
-    for (int u = 0; u < H; ++u) hist[u] = past && tid + 256 * u < a.history_stride ? h[tid + 256 * u] : 0;
+    for (int u = 0; u < H; ++u) hist[u] = past && tid + T * u < a.history_stride ? h[tid + T * u] : 0;
 #pragma unroll
-    for (int u = 0; u < B; ++u) bias[u] = a.bias_ids && tid + 256 * u < a.bias_stride ? ids[tid + 256 * u] : 0;
+    for (int u = 0; u < B; ++u) bias[u] = a.bias_ids && tid + T * u < a.bias_stride ? ids[tid + T * u] : 0;
     const uint32_t hist_len = past ? min(a.history_len[row], a.history_stride) : 0;
     const uint32_t bias_len = a.bias_ids ? min(a.bias_len[row], a.bias_stride) : 0;
     double rep = 1.0, pres = 0.0, freq = 0.0;
@@ -73,20 +74,20 @@ __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
         freq = a.penalties[3 * row + 2];
     }
 #pragma unroll
-    for (int q = 0; q < Q; ++q) *reinterpret_cast<uint4*>(named + 1024 * q + 4 * tid) = make_uint4(0, 0, 0, 0);
+    for (int q = 0; q < Q; ++q) *reinterpret_cast<uint4*>(named + 4 * (T * q + tid)) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     if (hist_len) {
         auto count = [&](uint32_t id, uint32_t i) {
             if (i < hist_len && id - base < n) atomicAdd(&named[id - base], 1u);
         };
 #pragma unroll
-        for (int u = 0; u < H; ++u) count(hist[u], tid + 256 * u);
-        for (uint32_t i0 = tid + 256 * H; i0 < hist_len; i0 += 1024) {
+        for (int u = 0; u < H; ++u) count(hist[u], tid + T * u);
+        for (uint32_t i0 = tid + T * H; i0 < hist_len; i0 += 4 * T) {
             uint32_t t[4];
 #pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) t[u] = i0 + 256 * u < hist_len ? h[i0 + 256 * u] : 0;
+            for (uint32_t u = 0; u < 4; ++u) t[u] = i0 + T * u < hist_len ? h[i0 + T * u] : 0;
 #pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) count(t[u], i0 + 256 * u);
+            for (uint32_t u = 0; u < 4; ++u) count(t[u], i0 + T * u);
         }
         __syncthreads();
     }
@@ -97,8 +98,8 @@ __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
             if (i < bias_len && id - base < n) atomicMax(&named[id - base], (i + 1) << 16 | (named[id - base] & 0xFFFFu));
         };
 #pragma unroll
-        for (int u = 0; u < B; ++u) note(bias[u], tid + 256 * u);
-        for (uint32_t i = tid + 256 * B; i < bias_len; i += 256) note(ids[i], i);
+        for (int u = 0; u < B; ++u) note(bias[u], tid + T * u);
+        for (uint32_t i = tid + T * B; i < bias_len; i += T) note(ids[i], i);
         __syncthreads();
     }
     float high = -INFINITY;  // of the thread's, its lowest token (they come in rising order)
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
     bool odd = false;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-        const uint32_t i = 1024 * q + 4 * tid;
+        const uint32_t i = 4 * (T * q + tid);
         const uint4 w4 = *reinterpret_cast<const uint4*>(named + i);
         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
         if (w4.x | w4.y | w4.z | w4.w)
@@ -144,17 +145,20 @@ __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
         __builtin_amdgcn_make_buffer_rsrc(a.part + (size_t)row * a.slices, 0, (int)(a.slices * 16), 0x00020000);
     uint32_t ticket = 0;
     if (tid == 0) {
-        for (int w = 1; w < 4; ++w) top = best[w] > top ? best[w] : top;
-        bad = worst[0] | worst[1] | worst[2] | worst[3];
+        bad = worst[0];
+        for (int w = 1; w < WAVES; ++w) {
+            top = best[w] > top ? best[w] : top;
+            bad |= worst[w];
+        }
         __builtin_amdgcn_raw_buffer_store_b128(v4u{(uint32_t)(top >> 32), (uint32_t)top, bad, 0u}, prs, part * 16, 0, kPartSC1);
         __builtin_amdgcn_s_waitcnt(kWaitVm0);
-        ticket = __hip_atomic_fetch_add(a.tickets + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        ticket = __hip_atomic_fetch_add(a.tickets + row * a.ticket_stride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if (a.out) {
         float* y = a.out + (size_t)row * a.out_stride + base;
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-            const uint32_t i = 1024 * q + 4 * tid;
+            const uint32_t i = 4 * (T * q + tid);
             if (VEC && i + 4 <= n)
                 *reinterpret_cast<float4*>(y + i) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
             else
@@ -179,7 +183,7 @@ __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
     if (tid == 0) {
         a.result[2 * row] = top >> 32 ? ~(uint32_t)top : 0xFFFFFFFFu;
         a.result[2 * row + 1] = found != 0;
-        __hip_atomic_store(a.tickets + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.tickets + row * a.ticket_stride, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
@@ -187,11 +191,12 @@ __global__ __launch_bounds__(256) void logits_select_kernel(LogitsSelect a) {
 
 hipError_t launch_logits_select(const LogitsSelect& a, hipStream_t s) {
     const bool vec = ((uintptr_t)a.logits | (uintptr_t)a.out) % 16 == 0 && a.stride % 4 == 0 && (!a.out || a.out_stride % 4 == 0);
-    const dim3 grid(a.rows * a.slices), block(256);
-    if (a.slice == 4096)
-        hipLaunchKernelGGL((vec ? logits_select_kernel<4, true> : logits_select_kernel<4, false>), grid, block, 0, s, a);
+    // few blocks: four times the threads, with a quarter of the work each
+    const dim3 grid(a.rows * a.slices);
+    if (grid.x >= 1024)
+        hipLaunchKernelGGL((vec ? logits_select_kernel<256, true> : logits_select_kernel<256, false>), grid, dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((vec ? logits_select_kernel<1, true> : logits_select_kernel<1, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((vec ? logits_select_kernel<1024, true> : logits_select_kernel<1024, false>), grid, dim3(1024), 0, s, a);
     return hipGetLastError();
 }
 

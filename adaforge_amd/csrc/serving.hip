@@ -299,7 +299,9 @@ int af_paged_attention(const af_paged_attention_args* p, void* stream) {
     a.b = batch_view(p->batch, p->pages);
     a.tickets = (uint32_t*)p->workspace->p;
     a.part = (float*)((char*)p->workspace->p + kTicketBytes);
-    const hipError_t e = launch_paged_attention(a, p->config.width, p->pages.type == AF_KV_Q4, attn_plan(shape_of(*p)), (hipStream_t)stream);
+    const AttnPlan plan = attn_plan(shape_of(*p));
+    a.ticket_stride = ticket_stride((uint64_t)plan.slots * a.kv_heads);
+    const hipError_t e = launch_paged_attention(a, p->config.width, p->pages.type == AF_KV_Q4, plan, (hipStream_t)stream);
     return e == hipSuccess ? AF_OK : fail(e, "paged attention launch");
 }
 
@@ -308,8 +310,7 @@ int af_logits_select_workspace(const af_logits_args* p, size_t* bytes) {
     if (p->rows == 0 || p->rows > AF_MAX_LOGIT_ROWS || p->vocabulary == 0 || p->vocabulary > 0x1000000u)
         return fail(AF_ERR_INVALID, "invalid number of rows or tokens of the vocabulary");
     if ((uint64_t)p->rows * p->vocabulary > 1ull << 34) return fail(AF_ERR_INVALID, "rows times vocabulary above 2^34");
-    const uint32_t slice = logits_slice(p->rows, p->vocabulary);
-    *bytes = kTicketBytes + (size_t)p->rows * ((p->vocabulary + slice - 1) / slice) * 16;
+    *bytes = kTicketBytes + (size_t)p->rows * ((p->vocabulary + kLogitsSlice - 1) / kLogitsSlice) * 16;
     return AF_OK;
 }
 
@@ -349,8 +350,8 @@ int af_logits_select(const af_logits_args* p, void* stream) {
     a.result = p->result;
     a.tickets = (uint32_t*)p->workspace->p;
     a.part = (uint4*)((char*)p->workspace->p + kTicketBytes);
-    a.slice = logits_slice(p->rows, p->vocabulary);
-    a.slices = (p->vocabulary + a.slice - 1) / a.slice;
+    a.ticket_stride = ticket_stride(p->rows);
+    a.slices = (p->vocabulary + kLogitsSlice - 1) / kLogitsSlice;
     const hipError_t e = launch_logits_select(a, (hipStream_t)stream);
     return e == hipSuccess ? AF_OK : fail(e, "logits launch");
 }
