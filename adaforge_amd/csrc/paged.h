@@ -149,6 +149,8 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     p.chunk = (tiles + splits - 1) / splits;
     p.splits = (tiles + p.chunk - 1) / p.chunk;
     const uint64_t row_bytes = (uint64_t)(a.width + 4) * 4;
+    // (many partial sums are stored, and joined, faster by many blocks of another launch: its partial sums need not go
+    // through to the memory side.  A prompt of 512 at 4,096 positions took 152 us joined by the last chunks, 111 apart.)
     p.join_apart = p.splits > 1 && (p.rows > 16 || p.splits * least(16, tokens * a.group) * row_bytes > 131072);
     p.part_bytes = p.splits > 1 ? (size_t)(sums * p.splits * p.rows * row_bytes) : 0;
     return p;

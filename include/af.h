@@ -242,7 +242,8 @@ size_t af_kv_page_bytes(uint32_t type, uint32_t page, uint32_t kv_heads, uint32_
  * every access in bounds whatever they hold.  A position without a page (a table entry that is not below
  * `pages`, a position at or past table_stride * page, a negative one where lengths[s] is less than the sequence's
  * rows) is not written and not seen, and reads as zeros; rows at or past starts[sequences] are left as they were.
- * starts rises from 0 to at most `tokens` (later rows of a larger start are cut off). */
+ * starts rises from 0 to at most `tokens` (later rows of a larger start are cut off); where it does not, rows and the
+ * workspace of the call may hold anything afterwards. */
 typedef struct {
     const uint32_t* starts;  /* device [sequences + 1] */
     const uint32_t* lengths; /* device [sequences]: positions cached, the batch's included */
@@ -289,7 +290,7 @@ int af_kv_read(const af_kv_pages* pages, const af_kv_batch* batch, uint16_t* k, 
  * position p sees every key j <= p of its sequence with window == 0, j > p - window, or j < sinks (the first
  * tokens that stay visible).  out = softmax(scale q.k) v per query head (q_heads / kv_heads of them share a KV
  * head), zeros where nothing is seen.  q as af_kv_append writes it; q and out rows are [q_heads][width] floats,
- * strides and alignment as there, out not overlapping q.  fp32 softmax and sums; the queries and probabilities enter
+ * strides and alignment as there, no row of out overlapping one of q.  fp32 softmax and sums; the queries and probabilities enter
  * the products with at least 22 significant bits.  longest_query (new tokens) and longest_context (length) of any
  * sequence are hints that only the split of the work, and the workspace's size, depend on: results are right
  * whatever they are, but one sequence may get slow where they are too small. */

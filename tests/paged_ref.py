@@ -140,27 +140,29 @@ def sees(p, j, window, sinks):
 def attention(batch, k, v, q, kv_heads, scale, window=0, sinks=0):
     """[tokens][q_heads][w] in 64 bits over page values k, v; rows that no sequence has are NaN."""
     tokens, qh, w = q.shape
-    out = np.full(q.shape, np.nan)
+    out, G = np.full(q.shape, np.nan), qh // kv_heads
     for s in range(len(batch.new)):
-        n = batch.lengths[s]
-        at = [batch.place(s, j) for j in range(max(0, n))]
-        held = np.array([a is not None for a in at], bool)
-        idx = [a for a in at if a is not None]
-        pg, sl = np.array([a[0] for a in idx], int), np.array([a[1] for a in idx], int)
+        n, new, first = batch.lengths[s], batch.new[s], int(batch.starts[s])
+        if new == 0:
+            continue
+        at = [(j, *batch.place(s, j)) for j in range(max(0, n)) if batch.place(s, j) is not None]
+        key, pg, sl = (np.array(c, int) for c in zip(*at)) if at else (np.zeros(0, int),) * 3
         K, V = k[pg, :, sl].astype(np.float64), v[pg, :, sl].astype(np.float64)
-        key = np.nonzero(held)[0]
-        for i in range(batch.new[s]):
-            p, row = n - batch.new[s] + i, int(batch.starts[s]) + i
-            m = sees(p, key, window, sinks) if key.size else np.zeros(0, bool)
-            if not m.any():
-                out[row] = 0.0
-                continue
-            for h in range(qh):
-                with np.errstate(all="ignore"):
-                    x = K[m, h * kv_heads // qh] @ q[row, h].astype(np.float64) * scale
-                    e = np.exp(x - x.max())
-                    keep = e != 0
-                    out[row, h] = (e[keep, None] * V[m, h * kv_heads // qh][keep]).sum(0) / e.sum()
+        pos = n - new + np.arange(new)
+        seen = sees(pos[:, None], key[None], window, sinks) & (pos[:, None] >= 0)
+        for h in range(qh):
+            with np.errstate(all="ignore"):
+                x = q[first:first + new, h].astype(np.float64) @ K[:, h // G].T * scale
+                x = np.where(seen, x, -np.inf)
+                top = x.max(1, initial=-np.inf, keepdims=True)
+                e = np.where(seen, np.exp(x - np.where(top == -np.inf, 0.0, top)), 0.0)
+                # a key without weight adds nothing, whatever its value
+                bad = ~np.isfinite(V[:, h // G]).all(1)
+                o = e[:, ~bad] @ V[~bad, h // G]
+                for j in np.nonzero(bad)[0]:
+                    o += np.where(e[:, j:j + 1] != 0, e[:, j:j + 1] * V[j, h // G], 0.0)
+                total = e.sum(1, keepdims=True)
+                out[first:first + new, h] = np.where(total == 0, 0.0, o / total)
     return out
 
 

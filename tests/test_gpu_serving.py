@@ -295,6 +295,86 @@ def test_attention_hints_do_not_change_what_is_computed(q4, new):
         assert (got[sum(new):] == -7).all()
 
 
+@pytest.mark.parametrize("q4,width", [(F16, 64), (Q4, 64), (F16, 256), (Q4, 256), (F16, 512), (Q4, 512)])
+@pytest.mark.parametrize("new", [[1], [30], [90]])
+def test_attention_over_many_chunks(q4, width, new):
+    """Contexts whose keys are split, for single tokens, several row tiles and shared tiles: 1 row of 90 or more at the end
+    of 3,000 positions, under a window of 1,500 with 40 first tokens too."""
+    _, b, kp, vp, q = make_attention(("chunks", int(q4), width, new[0]), q4, width, 64, 2, 1, new, [3000])
+    kv = kp.values(), vp.values()
+    for window, sinks in ((0, 0), (1500, 40)):
+        got, _ = run_attention(b, kp, vp, q, 1, window, sinks)
+        R.check_attention(got, R.attention(b, *kv, q, 1, 1 / np.sqrt(width), window, sinks), width, 2.0)
+
+
+@pytest.mark.parametrize("q4", [F16, Q4])
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("hint", [1, 20000])
+def test_long_chunks_and_many_of_them(q4, new, hint):
+    """One chunk of every key (the page numbers are read again and again), and as many as there may be (128)."""
+    _, b, kp, vp, q = make_attention(("long", int(q4), new), q4, 64, 16, 2, 1, [new], [20000])
+    got, _ = run_attention(b, kp, vp, q, 1, longest=(new, hint))
+    R.check_attention(got, R.attention(b, kp.values(), vp.values(), q, 1, 0.125), 64, 2.0)
+
+
+@pytest.mark.parametrize("q4", [F16, Q4])
+@pytest.mark.parametrize("sequences,longest", [(70, 3), (70, 60), (5000, 1)])
+def test_many_sequences(q4, sequences, longest):
+    """More sequences than one round of loads finds (64), some of them without rows."""
+    rng = rng_of("sequences", sequences, longest, int(q4))
+    new = [1] * sequences if longest == 1 else [int(rng.integers(0, 4)) for _ in range(sequences)]
+    if longest > 3:
+        new[3] = new[66] = longest
+    new[10] = 0
+    lengths = [n + int(rng.integers(0, 40)) for n in new]
+    _, b, kp, vp, q = make_attention(("sequences", sequences), q4, 64, 16, 4, 2, new, lengths)
+    want = R.attention(b, kp.values(), vp.values(), q, 2, 0.125)
+    got, _ = run_attention(b, kp, vp, q, 2)
+    R.check_attention(got, want, 64, 2.0)
+    k, v = f32(rng, b.tokens, 2, 64), f32(rng, b.tokens, 2, 64)
+    dev, _ = run_append(b, kp, vp, None, k, v, None, None, False, None)
+    rows = expected_append(b, None, k, v, None, None, False, None)
+    check_pool(dev.k, kp, b, rows, 1)
+    check_pool(dev.v, vp, b, rows, 2)
+
+
+def test_append_of_a_long_batch():
+    """Enough rows that a wave takes four of them."""
+    rng = rng_of("long batch")
+    for q4, width, qh, kv in ((F16, 128, 13, 2), (Q4, 64, 14, 1)):
+        b = R.Batch(rng, [1500, 600], [1500, 900], 64)
+        kp, vp = (R.Pool(rng, q4, b.pages, 64, kv, width) for _ in range(2))
+        q, k, v = (f32(rng, b.tokens, h, width) for h in (qh, kv, kv))
+        qn, kn = 1 + 0.1 * f32(rng, width), 1 + 0.1 * f32(rng, width)
+        turn = (1e4, np.ones(width // 2, np.float32))
+        dev, out = run_append(b, kp, vp, q, k, v, qn, kn, True, R.rope(width, *turn))
+        want = expected_append(b, q, k, v, qn, kn, True, turn)
+        for row, r in want.items():
+            f32_close(out[row], r[0])
+        if not q4:
+            check_pool(dev.k, kp, b, want, 1)
+            check_pool(dev.v, vp, b, want, 2)
+        else:  # (Pool.put packs a whole pool: the rows at once instead)
+            got = [R.Pool(rng, q4, b.pages, 64, kv, width) for _ in range(2)]
+            for g, buf, which in zip(got, (dev.k, dev.v), (1, 2)):
+                g.bytes[:] = buf.numpy()
+                w, d = g.planes()
+                for row, s, pos in b.rows():
+                    n, scale = R.quantise(want[row][which].astype(np.float32))
+                    pg, sl = b.place(s, pos)
+                    assert np.array_equal(((w[pg, :, sl, :, None] >> R.SHIFT) & 15).reshape(kv, width), n)
+                    assert np.array_equal(d[pg, :, sl], scale)
+
+
+def test_sequences_that_share_pages():
+    """A common beginning held once: both sequences' tables name its pages."""
+    for q4, new in ((F16, [1, 1]), (Q4, [40, 33])):
+        _, b, kp, vp, q = make_attention(("prefix", int(q4)), q4, 128, 16, 4, 2, new, [300, 250])
+        b.table[1, :12] = b.table[0, :12]
+        got, _ = run_attention(b, kp, vp, q, 2)
+        R.check_attention(got, R.attention(b, kp.values(), vp.values(), q, 2, 1 / np.sqrt(128)), 128, 2.0)
+
+
 @pytest.mark.parametrize("q4", [F16, Q4])
 @pytest.mark.parametrize("new", [[6, 3, 2, 1], [70, 80, 40, 66]])
 def test_attention_of_missing_keys(q4, new):
@@ -326,22 +406,28 @@ def test_unwritten_pages_are_never_seen(q4, new, window):
     R.check_attention(got, want, 64, 2.0)
 
 
-@pytest.mark.parametrize("new", [[1, 1], [45, 18]])
-@pytest.mark.parametrize("where", ["v", "k"])
-def test_an_infinity_reaches_only_the_positions_that_see_it(new, where):
-    """An overflowed value (fp16 infinity): queries before it are as without it, those that see it are as in plain
-    arithmetic (an infinite value in its channel; a key scored -infinity has no weight, one scored +infinity makes NaNs)."""
-    lengths = [60, 200]
-    rng, b, kp, vp, q = make_attention(("inf", new[0], where), F16, 64, 16, 2, 1, new, lengths)
+@pytest.mark.parametrize("new,before", [([1, 1], 0), ([45, 18], 0), ([1, 1], 1500), ([45, 18], 1500)])
+@pytest.mark.parametrize("where,value", [("v", np.inf), ("k", np.inf), ("k", -np.inf), ("v", np.nan), ("k", np.nan), ("q4 k", np.nan)])
+def test_an_infinity_reaches_only_the_positions_that_see_it(new, before, where, value):
+    """An overflowed value (an fp16 infinity, or a 4-bit block of NaNs): queries before it are as without it, those that
+    see it are as in plain arithmetic (an infinite value in its channel; a key scored -infinity has no weight, one scored
+    +infinity makes NaNs)."""
+    lengths = [before + 60, before + 200]
+    q4 = where.startswith("q4")
+    rng, b, kp, vp, q = make_attention(("inf", new[0], where[-1], before), q4, 64, 16, 2, 1, new, lengths)
     pool = vp if where == "v" else kp
-    at = b.place(0, 50 if new[0] > 1 else 20)
-    pool.planes()[0][at[0], 0, at[1], 7] = np.inf
+    at = b.place(0, before + (50 if new[0] > 1 else 20))
+    if q4:
+        codes, scales = pool.planes()
+        scales[at[0], 0, at[1], 1] = np.nan
+        pool._join(codes, scales)
+    else:
+        pool.planes()[0][at[0], 0, at[1], 7] = value
     got, _ = run_attention(b, kp, vp, q, 1)
     want = R.attention(b, kp.values(), vp.values(), q, 1, 0.125)
-    rows = ~np.isnan(want).all((1, 2)) | np.isnan(want).any((1, 2))
     fine = np.isfinite(want)
-    assert np.array_equal(np.isnan(want), np.isnan(got[:len(want)])) and np.array_equal(want == np.inf, got == np.inf)
-    assert rows.all() and not fine.all() or where == "k"
+    assert np.array_equal(np.isnan(want), np.isnan(got)) and np.array_equal(want == np.inf, got == np.inf)
+    assert fine.any()
     w = np.where(fine, want, 0.0)
     g = np.where(fine, got.astype(np.float64), 0.0)
     assert np.linalg.norm(g - w) <= 2 * R.attention_bound(64, 2.0) * np.linalg.norm(w)
@@ -530,6 +616,18 @@ def test_select_ids_twice_and_outside_the_vocabulary():
     got, ids = run_select(x, pen, hist, bias)
     same(got, want)
     assert np.array_equal(ids, result)
+
+
+@pytest.mark.parametrize("rows,vocab", [(64, 65536), (600, 5000), (1100, 130)])
+def test_select_many_rows(rows, vocab):
+    """Enough slices for the narrow blocks, more rows than tickets a line apart, rows of one slice."""
+    rng = rng_of("rows", rows)
+    x, pen, hist, bias, mask = select_inputs(rng, rows, vocab, 40, 5, 0.5)
+    want, result = R.select(x, pen, hist, bias, mask)
+    for _ in range(2):
+        got, ids = run_select(x, pen, hist, bias, mask)
+        same(got, want)
+        assert np.array_equal(ids, result)
 
 
 def test_select_longest_lists():
