@@ -116,16 +116,45 @@ AF_HD uint32_t longest_tiles(const AttnShape& a, uint32_t tokens) {
 
 constexpr uint32_t kManyRows = 64;
 
+// Chunks shared out by the work there is, not by the longest sequence: 2 to 64 sequences of row tiles of 16, whose key
+// tiles every block adds up for itself (a lane a sequence).  A KV head's chunks take `chunks` blocks at most (0: shared
+// out by the hints), of which those that fill the chip or even out what is left are `most`, and one a row tile
+// (`slots`).  32 conversations of 512 to 32,768 positions took 229 us by the longest and take 207 so, eight of 512-wide
+// heads 54 and 45, 16 of 64-wide ones 32 and 24; equal lengths lose what the addition costs, about 1 us a block: 16 at
+// 8,192 positions 96 and 98.
+struct Shares {
+    uint32_t most, chunks, slots;
+    uint32_t per_fill, per_safe, per_even;  // 2^32 over a number of chunks, rounded up: the blocks divide by multiplying
+};
+
+// x over the number of chunks (2 or more) that `per` belongs to, rounded up.
+AF_HD uint32_t per_chunk(uint32_t x, uint32_t per) { return (uint32_t)(((uint64_t)(x ? x - 1 : 0) * per) >> 32) + 1; }
+
+constexpr uint32_t kMaxParts = 128;
+
+// The key tiles of a chunk where the row tiles' key tiles come to `total`, `fill` chunks fill the chip and `even` even out.
+// Chunks of it are at most the larger number and one a row tile.
+AF_HD uint32_t share_of(uint32_t total, uint32_t per_fill, uint32_t per_even) {
+    return (least(most(4, per_chunk(total, per_fill)), most(32, per_chunk(total, per_even))) + 3) / 4 * 4;
+}
+
+// The chunk of a sequence of n key tiles: its share, but no small rest, and not above kMaxParts chunks.
+AF_HD uint32_t share_chunk(uint32_t share, uint32_t n) {
+    return n <= share + share / 2 ? most(n, 1) : most(share, (n + kMaxParts - 1) / kMaxParts);
+}
+
 // A launch: row tiles of `rows` rows, their keys in at most `splits` chunks of `chunk` tiles or more.  16 rows: grid
 // units (row tiles, sequences, KV heads) by splits; more: grid slots, KV heads and splits.
 struct AttnPlan {
     uint32_t rows, units, row_tiles, slots, splits, chunk;
     bool join_apart;  // the chunks are joined by a launch of their own
+    Shares shares;
     size_t part_bytes;
 };
 
 AF_HD AttnPlan attn_plan(const AttnShape& a) {
     AttnPlan p;
+    p.shares = Shares{0, 0, 0, 0, 0, 0};
     const uint32_t tokens = most(1, least(a.longest_query, a.tokens));
     const uint64_t pairs = (uint64_t)a.sequences * a.kv_heads;  // (at most 2^22: checked by the call)
     const uint32_t tiles = longest_tiles(a, tokens);
@@ -141,6 +170,12 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
         const uint32_t fill = least(most(1, 256 / p.units), (tiles + 3) / 4), even = least(most(1, 2048 / p.units), most(1, tiles / 32));
         splits = least(most(fill, even), 128);
         splits = sums > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / sums)));
+        if (a.sequences > 1 && a.sequences <= 64 && p.slots <= 512 && sums <= 2048 && tiles > 4) {
+            const uint32_t fill = most(2, 256 / a.kv_heads), safe = most(2, fill - least(fill, p.slots));
+            const uint32_t even = most(2, least(2048 / a.kv_heads, a.sequences * p.row_tiles * tiles / 32));
+            auto per = [](uint32_t n) { return (uint32_t)(((1ull << 32) + n - 1) / n); };
+            p.shares = Shares{most(fill, even), most(fill, even) + p.slots, p.slots, per(fill), per(safe), per(even)};
+        }
     } else {
         p.units = (uint32_t)sums;
         splits = most(least(most(1, 512 / p.units), most(1, tiles / 8)), least(most(1, 1024 / p.units), most(1, tiles / 16)));
@@ -153,6 +188,7 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     // through to the memory side.  A prompt of 512 at 4,096 positions took 152 us joined by the last chunks, 111 apart.)
     p.join_apart = p.splits > 1 && (p.rows > 16 || p.splits * least(16, tokens * a.group) * row_bytes > 131072);
     p.part_bytes = p.splits > 1 ? (size_t)(sums * p.splits * p.rows * row_bytes) : 0;
+    if (p.shares.chunks) p.part_bytes = (size_t)((uint64_t)p.shares.chunks * a.kv_heads * 16 * row_bytes);
     return p;
 }
 

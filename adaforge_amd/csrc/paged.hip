@@ -619,18 +619,18 @@ __device__ __forceinline__ void chunks_of(uint32_t tiles, uint32_t chunk, uint32
     parts = max(1u, (tiles + len - 1) / len);
 }
 
-// Rows c0, c0 + 4, .. of a row tile from its chunks' partial sums [parts][R][W + 4] (sums, maximum, sum of weights), a
-// row per wave: the chunks' weights first, a chunk per lane, then their sums, eight loads of a lane in flight and
+// Rows c0, c0 + 4 / S, .. of a row tile from its chunks' partial sums [parts][R][W + 4] (sums, maximum, sum of weights), S
+// waves a row: the chunks' weights first, a chunk per lane, then their sums, eight loads of a lane in flight and
 // in the order of the chunks.  parts: at most 128.
-template <int W>
-__device__ __forceinline__ void join_parts(const PagedAttn& a, const float* part, uint32_t splits, uint32_t parts, uint32_t R,
+template <int W, int S>
+__device__ __forceinline__ void join_parts(const PagedAttn& a, const float* part, uint32_t parts, uint32_t R,
                                            uint32_t c0, uint32_t nr, uint32_t row0, uint32_t first, uint32_t h) {
-    constexpr uint32_t L = W / 4 < 64 ? W / 4 : 64, G = 64 / L, K = W / 4 / L;  // lanes of a row, chunks side by side, quads of a lane
+    constexpr uint32_t Q = W / 4 / S, L = Q < 64 ? Q : 64, G = 64 / L, K = Q / L;  // a wave's quads, lanes of a row, chunks side by side, quads of a lane
     constexpr uint32_t U = 8 / K;                                               // chunks of a lane in flight
     const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, (int)(splits * R * (W + 4) * 4), 0x00020000);
-    const uint32_t lane = threadIdx.x & 63;
-    for (uint32_t c = c0 + wave_id(); c < nr; c += 4) {
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part), 0, (int)(parts * R * (W + 4) * 4), 0x00020000);
+    const uint32_t lane = threadIdx.x & 63, x0 = wave_id() % S * Q;
+    for (uint32_t c = c0 + wave_id() / S; c < nr; c += 4 / S) {
         v4u v[U][K];
         auto load = [&](uint32_t q0) {
 #pragma unroll
@@ -638,7 +638,7 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, const float* part
 #pragma unroll
                 for (uint32_t k = 0; k < K; ++k)
                     v[u][k] = __builtin_amdgcn_raw_buffer_load_b128(
-                        rs, ((min(q0 + lane / L + u * G, parts - 1) * R + c) * (W + 4) + (lane % L + L * k) * 4) * 4, 0, kPartSC1);
+                        rs, ((min(q0 + lane / L + u * G, parts - 1) * R + c) * (W + 4) + (x0 + lane % L + L * k) * 4) * 4, 0, kPartSC1);
         };
         u2 ml[2];
 #pragma unroll
@@ -680,7 +680,7 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, const float* part
         if (lane < L)
 #pragma unroll
             for (uint32_t k = 0; k < K; ++k)
-                *reinterpret_cast<f4*>(out + (lane + L * k) * 4) = sum == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o[k] / sum;
+                *reinterpret_cast<f4*>(out + (x0 + lane + L * k) * 4) = sum == 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : o[k] / sum;
     }
 }
 
@@ -698,19 +698,98 @@ __device__ __forceinline__ bool last_chunk(const PagedAttn& a, uint32_t unit, ui
     return last;
 }
 
+// Sums over the lanes up to this one: within rows of 16 by shifts, then a row's last lane to the next row, lane 31's to the
+// upper half.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);  // row_shr by 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+    return v;
+}
+
+// n / d for n below 2^23, d > 0, rounded down.
+__device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d) {
+    uint32_t q = (uint32_t)((float)n * __builtin_amdgcn_rcpf((float)d));  // (off by at most one)
+    const int32_t rest = (int32_t)(n - q * d);
+    return rest < 0 ? q - 1 : (uint32_t)rest >= d ? q + 1 : q;
+}
+
+// A sequence's part of what Shares deals out: `parts` chunks of `chunk` key tiles for each of its row tiles, the first
+// of them chunk `first` of a KV head's.
+struct Share {
+    uint32_t seq, start, chunk, parts, first;
+    Span s;
+};
+
+// The sequence for whose lane find(start, span, its first chunk, the end of its chunks) is true, or false.
+template <typename F>
+__device__ __forceinline__ bool share(const PagedAttn& a, const Shares& sh, Share& o, F find) {
+    const uint32_t lane = threadIdx.x & 63, i = min(lane, a.b.sequences - 1);
+    const uint32_t start = *gp(a.b.starts + i), stop = *gp(a.b.starts + i + 1), length = *gp(a.b.lengths + i);
+    const Span s = span_of(start, stop, length, a.b);
+    const uint32_t r = lane < a.b.sequences ? (s.count * a.group + 15) / 16 : 0;
+    const uint32_t n = r ? tiles_of<32>(s.pos0, s.pos0 + (int32_t)s.count - 1, s.end, a.window, a.sinks).count : 0;
+    const uint32_t row_tiles = __builtin_amdgcn_readlane(wave_prefix(r), 63), total = __builtin_amdgcn_readlane(wave_prefix(r * n), 63);
+    if (row_tiles > sh.slots) return false;  // (starts that do not rise)
+    uint32_t chunk, c, end;  // key tiles of the lane's chunks, chunks of a row tile, end of all of them
+    auto deal = [&](uint32_t per_fill) {
+        chunk = share_chunk(share_of(total, per_fill, sh.per_even), n);
+        c = max(1u, quotient(n + chunk - 1, chunk));
+        end = wave_prefix(r * c);
+        return (uint32_t)__builtin_amdgcn_readlane(end, 63);
+    };
+    // (equal lengths share evenly; others leave each row tile a smaller last chunk, and fill the chip with fewer)
+    if (deal(sh.per_fill) > sh.most) deal(sh.per_safe);
+    const uint64_t mine = __ballot(find(start, s, end - r * c, end));
+    if (!mine) return false;
+    const uint32_t l = __builtin_ctzll(mine);
+    auto at = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); };
+    o.seq = l;
+    o.start = at(start);
+    o.s = span_of(o.start, at(stop), at(length), a.b);
+    o.chunk = at(chunk);
+    o.parts = at(c);
+    o.first = at(end - r * c);
+    return true;
+}
+
 // join_apart: the chunks are joined by paged_join_kernel afterwards, not by the last of them.
 template <int W, bool Q4, bool NT>
 __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedAttn a, uint32_t units, uint32_t splits,
-                                                                          uint32_t row_tiles, uint32_t chunk, bool join_apart) {
+                                                                          uint32_t row_tiles, uint32_t chunk, bool join_apart,
+                                                                          Shares shares) {
     constexpr int ST = W / 32, TV = W / 16, HALFROWS = 8;
     using V = VHalf<W, Q4, NT>;
     __shared__ __align__(16) uint8_t lds[W * 128];  // the queries' operands; at the end eight rows of each wave's sums
     __shared__ float wm[4][16], wl[4][16];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, g = lane >> 4;
-    const uint32_t split = blockIdx.x / units, unit = blockIdx.x % units;
-    const uint32_t h = unit % a.kv_heads, seq = unit / a.kv_heads % a.b.sequences, tile0 = unit / a.kv_heads / a.b.sequences;
-    const uint32_t start = a.b.starts[seq];
-    const Span s = span_of(start, a.b.starts[seq + 1], a.b.lengths[seq], a.b);
+    uint32_t h, seq, tile0, split, start, part0 = 0;  // part0: of the row tile's chunks, in shares
+    Span s;
+    if (shares.chunks) {
+        h = blockIdx.x % a.kv_heads;
+        const uint32_t b = blockIdx.x / a.kv_heads;
+        Share o;
+        if (!share(a, shares, o, [&](uint32_t, const Span&, uint32_t first, uint32_t end) { return b >= first && b < end; })) return;
+        seq = o.seq;
+        start = o.start;
+        s = o.s;
+        chunk = o.chunk;
+        const uint32_t r = (s.count * a.group + 15) / 16;
+        split = __builtin_amdgcn_readfirstlane(quotient(b - o.first, r));
+        tile0 = b - o.first - split * r;  // (a chunk's row tiles one after another: its K and V come from memory once)
+        part0 = h * shares.chunks + o.first + tile0 * o.parts;
+    } else {
+        split = blockIdx.x / units;
+        const uint32_t unit = blockIdx.x % units;
+        h = unit % a.kv_heads;
+        seq = unit / a.kv_heads % a.b.sequences;
+        tile0 = unit / a.kv_heads / a.b.sequences;
+        start = a.b.starts[seq];
+        s = span_of(start, a.b.starts[seq + 1], a.b.lengths[seq], a.b);
+    }
     const uint32_t rows = s.count * a.group;
 
     // (one turn unless a sequence has more rows than the launch was told)
@@ -873,7 +952,8 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         // the waves' sums meet in LDS, eight rows at a time
         float* sums = reinterpret_cast<float*>(lds);  // [wave][row of 8][W]
         const uint32_t slot = (start * a.group / 16 + seq + rt) * a.kv_heads + h;
-        float* part = a.part + ((size_t)slot * splits + split) * 16 * (W + 4);
+        float* parts0 = a.part + (shares.chunks ? (size_t)part0 : (size_t)slot * splits) * 16 * (W + 4);
+        float* part = parts0 + (size_t)split * 16 * (W + 4);
         __syncthreads();  // every wave is past its queries
         if (lane < 16) {
             wm[wave][m] = sm.m;
@@ -936,7 +1016,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
             }
         }
         if (parts > 1 && !join_apart && last_chunk(a, slot, parts))
-            join_parts<W>(a, a.part + (size_t)slot * splits * 16 * (W + 4), splits, parts, 16, 0, nr, rt * 16, s.first, h);
+            join_parts<W, 1>(a, parts0, parts, 16, 0, nr, rt * 16, s.first, h);
     }
 }
 
@@ -948,14 +1028,30 @@ __device__ __forceinline__ uint32_t slot_sequence(const PagedAttn& a, uint32_t s
     return seq;
 }
 
-// Joins the chunks of (row tile, KV head) slots, a block per four rows, so that wide tiles of many chunks are read by
+// Joins the chunks of (row tile, KV head) slots, a block per 4 / S rows, so that wide tiles of many chunks are read by
 // many CUs.
-template <int W>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t splits, uint32_t chunk, uint32_t R) {
-    const uint32_t groups = R / 4, slot = blockIdx.x / groups, c0 = blockIdx.x % groups * 4, h = slot % a.kv_heads;
+template <int W, int S>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t splits, uint32_t chunk, uint32_t R, Shares shares) {
+    const uint32_t groups = R * S / 4, slot = blockIdx.x / groups, c0 = blockIdx.x % groups * (4 / S), h = slot % a.kv_heads;
     uint32_t tile;
     Span s;
-    slot_sequence(a, slot / a.kv_heads, R, tile, s);
+    const float* part = a.part + (size_t)slot * splits * R * (W + 4);
+    if (shares.chunks) {
+        Share o;  // (the last sequence whose slots begin at or before this one)
+        const uint32_t at = slot / a.kv_heads;
+        if (!share(a, shares, o, [&](uint32_t start, const Span& s, uint32_t first, uint32_t end) {
+                const uint32_t base = s.first * a.group / 16 + (threadIdx.x & 63);
+                return end > first && at >= base && at < base + (s.count * a.group + 15) / 16;
+            }))
+            return;
+        s = o.s;
+        chunk = o.chunk;
+        splits = kMaxParts;
+        tile = at - (o.start * a.group / 16 + o.seq);
+        part = a.part + (size_t)(h * shares.chunks + o.first + tile * o.parts) * R * (W + 4);
+    } else {
+        slot_sequence(a, slot / a.kv_heads, R, tile, s);
+    }
     const uint32_t rows = s.count * a.group;
     if (tile * R >= rows) return;
     const uint32_t nr = min(R, rows - tile * R);
@@ -965,7 +1061,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
     uint32_t len, parts;
     chunks_of(keys.count, chunk, splits, len, parts);
     if (parts == 1) return;
-    join_parts<W>(a, a.part + (size_t)slot * splits * R * (W + 4), splits, parts, R, c0, min(nr, c0 + 4), tile * R, s.first, h);
+    join_parts<W, S>(a, part, parts, R, c0, min(nr, c0 + 4 / S), tile * R, s.first, h);
 }
 
 // ---- attention of many rows: prompts and further turns --------------------------------------------------
@@ -1432,16 +1528,20 @@ hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, c
     return by_layout(width, q4, [&](auto w, auto t) {
         constexpr int W = decltype(w)::value;
         constexpr bool Q4 = decltype(t)::value;
-        const dim3 grid(p.units * p.splits), block(256);
+        const dim3 grid(p.shares.chunks ? p.shares.chunks * a.kv_heads : p.units * p.splits), block(256);
         if (p.rows == 16) {
             hipLaunchKernelGGL((p.row_tiles == 1 ? paged_few_kernel<W, Q4, !Q4> : paged_few_kernel<W, Q4, false>), grid, block, 0, s, a,
-                               p.units, p.splits, p.row_tiles, p.chunk, p.join_apart);
+                               p.units, p.shares.chunks ? kMaxParts : p.splits, p.shares.chunks ? p.slots : p.row_tiles, p.chunk,
+                               p.join_apart, p.shares);
         } else {
             hipLaunchKernelGGL((paged_many_kernel<W, Q4>), grid, block, 0, s, a, p.slots, p.splits, p.chunk);
         }
         hipError_t e = hipGetLastError();
         if (e == hipSuccess && p.join_apart) {
-            hipLaunchKernelGGL(paged_join_kernel<W>, dim3(p.slots * a.kv_heads * (p.rows / 4)), block, 0, s, a, p.splits, p.chunk, p.rows);
+            // (few rows have many chunks: read by all waves of a block.  52 chunks of 512-wide heads took 12 us by one, 7 by four)
+            const uint32_t waves = p.rows == 16 ? 4 : 1;
+            hipLaunchKernelGGL((waves == 4 ? paged_join_kernel<W, 4> : paged_join_kernel<W, 1>),
+                               dim3(p.slots * a.kv_heads * (p.rows * waves / 4)), block, 0, s, a, p.splits, p.chunk, p.rows, p.shares);
             e = hipGetLastError();
         }
         return e;

@@ -317,6 +317,22 @@ def test_long_chunks_and_many_of_them(q4, new, hint):
     R.check_attention(got, R.attention(b, kp.values(), vp.values(), q, 1, 0.125), 64, 2.0)
 
 
+@pytest.mark.parametrize("q4,width", [(F16, 64), (Q4, 128), (Q4, 256), (F16, 512)])
+@pytest.mark.parametrize("new,lengths", [([1, 1], [2500, 30]), ([1, 0, 1, 1, 1], [200, 900, 0, 3000, 1400]),
+                                         ([6, 25, 1, 0, 9], [1000, 2600, 1, 50, 9]), ([1] * 64, [1 + 37 * i for i in range(64)])])
+def test_sequences_of_very_different_lengths(q4, width, new, lengths):
+    """Chunks dealt out by the lengths there are: long beside short and empty ones, one and several row tiles, one more row
+    behind the last sequence; with a window too."""
+    _, b, kp, vp, q = make_attention(("ragged", int(q4), width, len(new), new[0]), q4, width, 16, 2, 1, new, lengths, tokens=sum(new) + 1)
+    kv = kp.values(), vp.values()
+    for window, sinks in ((0, 0), (700, 40)):
+        want = R.attention(b, *kv, q, 1, 1 / np.sqrt(width), window, sinks)
+        for longest in ((max(new), max(lengths)), (1, 300)):
+            got, _ = run_attention(b, kp, vp, q, 1, window, sinks, longest)
+            R.check_attention(got, want, width, 2.0)
+            assert (got[sum(new):] == -7).all()
+
+
 @pytest.mark.parametrize("q4", [F16, Q4])
 @pytest.mark.parametrize("sequences,longest", [(70, 3), (70, 60), (5000, 1)])
 def test_many_sequences(q4, sequences, longest):
