@@ -95,6 +95,7 @@ inline uint32_t ticket_stride(uint64_t count) {
 struct AttnShape {
     uint32_t sequences, tokens, kv_heads, group, width, window, sinks;
     uint32_t longest_query, longest_context, capacity;  // (capacity: positions a page table row holds)
+    bool q4;
 };
 
 // Row tiles' slots for partial sums: sequence s's tiles start at slot starts[s] group / R + s, so every sequence's lie
@@ -119,7 +120,7 @@ constexpr uint32_t kManyRows = 64;
 // Chunks shared out by the work there is, not by the longest sequence: 2 to 64 sequences of row tiles of 16, whose key
 // tiles every block adds up for itself (a lane a sequence).  A KV head's chunks take `chunks` blocks at most (0: shared
 // out by the hints), of which those that fill the chip or even out what is left are `most`, and one a row tile
-// (`slots`).  32 conversations of 512 to 32,768 positions took 229 us by the longest and take 207 so, eight of 512-wide
+// (`slots`).  32 conversations of 1 to 8,192 positions took 229 us by the longest and take 205 so, eight of 512-wide
 // heads 54 and 45, 16 of 64-wide ones 32 and 24; equal lengths lose what the addition costs, about 1 us a block: 16 at
 // 8,192 positions 96 and 98.
 struct Shares {
@@ -159,14 +160,20 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     const uint64_t pairs = (uint64_t)a.sequences * a.kv_heads;  // (at most 2^22: checked by the call)
     const uint32_t tiles = longest_tiles(a, tokens);
     p.row_tiles = (uint32_t)(((uint64_t)tokens * a.group + 15) / 16);
-    p.rows = p.row_tiles > 4 ? kManyRows : 16;
+    // Up to four row tiles of 16 read K and V once each (from an L2), more share them through LDS, 64 rows at a time.  Eight
+    // sequences of 4,096 positions, 256-wide 4-bit heads: three tiles 72 us, by 64 rows 87, four 89 and 98, five 110 and
+    // 111, eight 168 and 138.  256-wide fp16 rows, which need the most from the L2, share from three tiles on once there
+    // are key tiles enough to fill the chip: three sequences of 4,096 positions 63 us and 47, eight of 1,000 34 and 37.
+    const bool heavy = !a.q4 && a.width == 256 && pairs * tiles > 2048;
+    p.rows = p.row_tiles > (heavy ? 2u : 4u) ? kManyRows : 16;
     p.slots = row_slots(a, p.rows);
     if (p.row_tiles * pairs > 1u << 22) p.row_tiles = most(1, (uint32_t)((1u << 22) / pairs));
     const uint64_t sums = (uint64_t)p.slots * a.kv_heads;
     uint32_t splits;
     if (p.rows == 16) {
         p.units = (uint32_t)(p.row_tiles * pairs);
-        // as many chunks as fill the chip, then more of at least 32 tiles for lengths that differ
+        // as many chunks as fill the chip, then more of at least 32 tiles for lengths that differ (32 conversations of up
+        // to 8,192 positions 205 us, of 64 tiles 217; eight of 512-wide heads 44, of 16 tiles 70)
         const uint32_t fill = least(most(1, 256 / p.units), (tiles + 3) / 4), even = least(most(1, 2048 / p.units), most(1, tiles / 32));
         splits = least(most(fill, even), 128);
         splits = sums > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / sums)));
@@ -178,6 +185,7 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
         }
     } else {
         p.units = (uint32_t)sums;
+        // two blocks a CU (a prompt of 512 rows in chunks of 8 tiles 30 us, of 4 tiles 33), or four of longer chunks
         splits = most(least(most(1, 512 / p.units), most(1, tiles / 8)), least(most(1, 1024 / p.units), most(1, tiles / 16)));
         splits = least(splits, 16);
     }

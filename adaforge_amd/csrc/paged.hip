@@ -97,7 +97,9 @@ __device__ __forceinline__ void unpack4(uint32_t w, _Float16 d, h2 (&o)[4]) {
 // f32, and for K and V the cache's type.  An angle is position times turns mod 2^64 as a fraction of a turn: a
 // product that wraps keeps exactly the part that sine and cosine see, so far positions lose nothing and no general
 // argument reduction is needed.  Its rows are on their way while the token's place is looked up.  N = 4 shares the sines
-// among four rows and keeps four times the bytes in flight; N = 1 spreads a decode step over the chip.
+// among four rows and keeps four times the bytes in flight; N = 1 spreads a decode step over the chip.  Bound by 8 bytes
+// per value of q, 4 and the cache's per value of k and v: four prompts (1,820 rows of 16 + 16 heads, 105 MB) 28.5 us =
+// 3.7 TB/s, N = 1 45 us; by latency where there are few: one token 3.4 us, 64 tokens to 4 bits 6.3, N = 4 13.
 
 template <int W, bool Q4, int N>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppend a, uint32_t groups, uint32_t tasks) {
@@ -349,7 +351,11 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
 // Rows are the (token, query head) pairs that share a KV head: row i of a sequence is token i / group, head i % group.
 // A block takes 16 of them against a chunk of the sequence's key tiles, its four waves tile by tile in turn; the
 // chunks of one row tile meet at a ticket, where the last block joins their partial sums (one pass over the
-// data with a running maximum and sum).  Bound by reading K and V once.
+// data with a running maximum and sum).  Bound by reading K and V once: one token at 32,768 positions (8 heads of 256,
+// fp16, 268 MB) 50.6 us = 5.3 TB/s, 32 of 1 to 8,192 positions 204 us = 5.3 TB/s; 4-bit rows by unpacking them (13
+// instructions a word of eight) and by the waits between dependent steps: 64 windows of 1,024 41.8 us = 3.6 TB/s, eight
+// 512-wide heads of up to 32,768 positions (a block a CU) 38 us and 7 the join; short contexts by the chain of the
+// sequence's place, the page numbers, K, V, the ticket and the join: one token at 512 positions 10.6 us.
 //
 // Products are taken transposed on the fp16 matrix cores, S^T = K Q^T and O^T = V^T P^T (16 keys or channels by 16
 // rows): a lane holds one row's column throughout (row lane % 16), so the softmax needs two lane swaps per
@@ -1069,7 +1075,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
 // Row tiles of 64 rows: a wave holds 16 of them from scores to output, their queries and sums in registers, and
 // the block's four waves share K and V through LDS, 32 keys at a time in two buffers: while one tile is used, the next
 // one is on its way (in registers, then in the other buffer) and one barrier separates tiles.  Bound by the matrix
-// cores' 8 W multiply-adds per (row, key): both operands' pairs double the 4 W of the product.
+// cores' 8 W operations per (row, key): both operands' pairs double the 4 W of the two products.  Eight chunks of 512
+// tokens at 4,096 positions (16 heads of 256): 530 us fp16, 560 4-bit, 960 TFLOP/s of pairs, 0.89 of what a large
+// fp16 product reaches here; one prompt of 512, whose blocks take 8 tiles each, 22 us and 8 the join.
+// Slower: 32 rows a wave (one wave a SIMD: 763 us against 586 at that step), the last chunk's block joining (152 against
+// 111 us for one chunk of 512).
 //
 // K lies in LDS as the first product reads it, piece ((half, step), lane) of 16 bytes; V transposed, piece (tile of 16
 // channels, lane), its channels ordered by their place in an octet (E values of a load), so that both what a wave

