@@ -174,7 +174,8 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
         p.units = (uint32_t)(p.row_tiles * pairs);
         // as many chunks as fill the chip, then more of at least 32 tiles for lengths that differ (32 conversations of up
         // to 8,192 positions 205 us, of 64 tiles 217; eight of 512-wide heads 44, of 16 tiles 70)
-        const uint32_t fill = least(most(1, 256 / p.units), (tiles + 3) / 4), even = least(most(1, 2048 / p.units), most(1, tiles / 32));
+        const uint32_t fill = least(most(1, 256 / p.units), (tiles + 3) / 4);
+        const uint32_t even = least(most(1, 2048 / p.units), most(1, tiles / 32));
         splits = least(most(fill, even), 128);
         splits = sums > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / sums)));
         if (a.sequences > 1 && a.sequences <= 64 && p.slots <= 512 && sums <= 2048 && tiles > 4) {

@@ -200,10 +200,11 @@ int af_attention_decode(const af_attention_args* args, void* stream);
  *      (no counterpart in the reference, which decodes one sequence over contiguous buffers) --------- */
 
 /* Device memory that calls use between their launches' blocks: completion tickets (zero between calls) and
- * partial results.  A call checks that its workspace is large enough (the *_workspace functions say how large:
- * any call of the same sizes or smaller ones fits, of either kind) and on its stream's device.  Calls that share
- * one must not overlap: give each stream, and each captured graph that may run beside another, its own.  It
- * lives on the device current when it is created and must outlive the graphs captured with it. */
+ * partial results.  A call checks that its workspace is large enough (the *_workspace functions say how large for
+ * its sizes; one workspace serves calls of either kind) and on its stream's device.  Fewer or shorter sequences may
+ * need more than many, split more: one of 65536 + 524288 * (width + 4) bytes fits every attention of its head width.
+ * Calls that share one must not overlap: give each stream, and each captured graph that may run beside another,
+ * its own.  It lives on the device current when it is created and must outlive the graphs captured with it. */
 typedef struct af_workspace af_workspace;
 int af_workspace_create(size_t bytes, af_workspace** out);
 void af_workspace_free(af_workspace* w);

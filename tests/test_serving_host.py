@@ -99,6 +99,22 @@ def test_attention_workspace_asks_for_sizes_alone():
     refused(N.lib().af_paged_attention_workspace(ctypes.byref(attention_args()), None))
 
 
+def test_one_workspace_fits_every_attention_of_a_width():
+    rng, need = random.Random(6), ctypes.c_size_t()
+    pick = lambda *c: rng.choice(c)
+    for _ in range(20000):
+        width, kv = pick(64, 128, 256, 512), pick(1, 2, 3, 8, 16, 100, 1024)
+        group = pick(1, 2, 5, 16, 1024 // kv) if kv < 1024 else 1
+        qh = kv * group if kv * group <= 1024 else kv
+        b = batch(sequences=pick(1, 2, 3, 8, 64, 65, 1000, 4096, rng.randint(1, 4096)), tokens=pick(1, 4, 64, 512, 65536, rng.randint(1, 65536)),
+                  table_stride=pick(1, 100, 1 << 16))
+        a = attention_args(p=pages(kv_heads=kv, width=width, type=pick(N.AF_KV_F16, N.AF_KV_Q4), page=16), b=b,
+                           config=(qh, kv, width, pick(0, 1, 1024), 0.125), sinks=pick(0, 4),
+                           longest_query=pick(0, 1, 16, 600, 0xFFFFFFFF), longest_context=pick(0, 1, 500, 8192, 0xFFFFFFFF))
+        assert N.lib().af_paged_attention_workspace(ctypes.byref(a), ctypes.byref(need)) == N.AF_OK
+        assert need.value <= 65536 + 524288 * (width + 4)
+
+
 def logits_args(**kw):
     d = dict(logits=A, stride=100, out=None, out_stride=0, rows=2, vocabulary=100, penalties=A, history=A, history_stride=5,
              history_len=A, bias_ids=A, bias_values=A, bias_stride=5, bias_len=A, mask=A, mask_stride=4, result=A,
