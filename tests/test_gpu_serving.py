@@ -763,6 +763,53 @@ def test_serving_steps_captured_and_replayed(q4):
         assert np.array_equal(outs[1][2], result)
 
 
+@pytest.mark.parametrize("q4,width", [(F16, 256), (Q4, 128)])
+def test_captured_attention_follows_the_lengths(q4, width):
+    """One graph, replayed over lengths that deal the chunks out quite differently, sequences without rows among them."""
+    longest, kv, qh = 4000, 2, 4
+    _, b, kp, vp, q = make_attention(("replay", int(q4)), q4, width, 32, qh, kv, [1] * 6, [longest] * 6)
+    dev, qb, o, stream = R.Device(b, kp, vp), up(q), up(np.zeros(q.shape, np.float32)), hip.Stream()
+    args = R.attend_args(dev, qb, o, qh, 1 / np.sqrt(width), 0, 0, (1, longest))
+    size = N.sz()
+    N.check(N.lib().af_paged_attention_workspace(ctypes.byref(args), ctypes.byref(size)))
+    ws = R.workspace(size.value)
+    args.workspace = ws.h
+    graph = hip.Graph(stream, lambda: N.check(N.lib().af_paged_attention(ctypes.byref(args), stream.handle)))
+    values = kp.values(), vp.values()
+    for lengths in ([longest] * 6, [1, 2, 3, 4, 5, 6], [longest, 1, 1, 1, 1, 1], [40, 3999, 0, 700, 0, 64], [longest] * 6, [0] * 6):
+        dev.keep[1].upload(np.array(lengths, np.uint32))
+        o.upload(np.full(q.shape, -7, np.float32))
+        graph.launch(stream)
+        stream.synchronize()
+        got = o.numpy()
+        o.upload(np.full(q.shape, -7, np.float32))
+        N.check(N.lib().af_paged_attention(ctypes.byref(args), None))
+        hip.synchronize()
+        assert np.array_equal(got.view(np.uint32), o.numpy().view(np.uint32)), lengths
+        now = R.Batch.__new__(R.Batch)
+        now.__dict__ = {**b.__dict__, "lengths": lengths}
+        R.check_attention(got, R.attention(now, *values, q, kv, 1 / np.sqrt(width), 0, 0), width, 2.0)
+
+
+def test_attention_of_arrays_that_do_not_rise_stays_inside():
+    """starts that fall, rows named by several sequences, lengths past the table: the pools stay as they are, rows behind
+    the batch too, and a fresh workspace serves the next call."""
+    _, b, kp, vp, q = make_attention(("falls",), Q4, 64, 16, 4, 2, [3] * 5, [900, 10, 500, 700, 3], tokens=20)
+    want = R.attention(b, kp.values(), vp.values(), q, 2, 0.125)
+    for starts, lengths in (([0, 15, 0, 15, 0, 15], [900, 900, 900, 900, 900]), ([15, 12, 9, 6, 3, 0], [1 << 31] * 5),
+                            ([0, 0xFFFFFFFF, 2, 0xFFFFFFFF, 4, 5], [900, 0, 0xFFFFFFFF, 7, 900]), ([20] * 6, [900] * 5)):
+        dev, qb = R.Device(b, kp, vp), up(q)
+        dev.keep[0].upload(np.array(starts, np.uint32))
+        dev.keep[1].upload(np.array(lengths, np.uint32))
+        o = up(np.full(q.shape, -7, np.float32))
+        R.attend(dev, qb, o, 4, 0.125, longest=(3, 900))
+        o.numpy()
+        assert np.array_equal(dev.k.numpy(), kp.bytes) and np.array_equal(dev.v.numpy(), vp.bytes)
+    got, _ = run_attention(b, kp, vp, q, 2)
+    R.check_attention(got, want, 64, 2.0)
+    assert (got[15:] == -7).all()
+
+
 def test_two_streams_with_a_workspace_each():
     rng, b, kp, vp, q = make_attention(("streams",), F16, 256, 16, 4, 2, [1, 1], [5000, 3000])
     want = R.attention(b, kp.values(), vp.values(), q, 2, 1 / 16)
