@@ -117,8 +117,8 @@ AF_HD uint32_t longest_tiles(const AttnShape& a, uint32_t tokens) {
 
 constexpr uint32_t kManyRows = 64;
 
-// Chunks shared out by the work there is, not by the longest sequence: 2 to 64 sequences of row tiles of 16, whose key
-// tiles every block adds up for itself (a lane a sequence).  A KV head's chunks take `chunks` blocks at most (0: shared
+// Chunks shared out by the work there is, not by the longest sequence: 2 to 64 sequences, whose key tiles every block adds up
+// for itself (a lane a sequence).  A KV head's chunks take `chunks` blocks at most (0: shared
 // out by the hints), of which those that fill the chip or even out what is left are `most`, and one a row tile
 // (`slots`).  32 conversations of 1 to 8,192 positions took 229 us by the longest and take 205 so, eight of 512-wide
 // heads 54 and 45, 16 of 64-wide ones 32 and 24; equal lengths lose what the addition costs, about 1 us a block: 16 at
@@ -126,6 +126,7 @@ constexpr uint32_t kManyRows = 64;
 struct Shares {
     uint32_t most, chunks, slots;
     uint32_t per_fill, per_safe, per_even;  // 2^32 over a number of chunks, rounded up: the blocks divide by multiplying
+    uint32_t few, some;                    // key tiles that a chunk has at least, where it fills the chip, and where it evens out
 };
 
 // x over the number of chunks (2 or more) that `per` belongs to, rounded up.
@@ -135,8 +136,8 @@ constexpr uint32_t kMaxParts = 128;
 
 // The key tiles of a chunk where the row tiles' key tiles come to `total`, `fill` chunks fill the chip and `even` even out.
 // Chunks of it are at most the larger number and one a row tile.
-AF_HD uint32_t share_of(uint32_t total, uint32_t per_fill, uint32_t per_even) {
-    return (least(most(4, per_chunk(total, per_fill)), most(32, per_chunk(total, per_even))) + 3) / 4 * 4;
+AF_HD uint32_t share_of(const Shares& s, uint32_t total, uint32_t per_fill) {
+    return (least(most(s.few, per_chunk(total, per_fill)), most(s.some, per_chunk(total, s.per_even))) + 3) / 4 * 4;
 }
 
 // The chunk of a sequence of n key tiles: its share, but no small rest, and not above kMaxParts chunks.
@@ -155,7 +156,7 @@ struct AttnPlan {
 
 AF_HD AttnPlan attn_plan(const AttnShape& a) {
     AttnPlan p;
-    p.shares = Shares{0, 0, 0, 0, 0, 0};
+    p.shares = Shares{};
     const uint32_t tokens = most(1, least(a.longest_query, a.tokens));
     const uint64_t pairs = (uint64_t)a.sequences * a.kv_heads;  // (at most 2^22: checked by the call)
     const uint32_t tiles = longest_tiles(a, tokens);
@@ -178,17 +179,24 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
         const uint32_t even = least(most(1, 2048 / p.units), most(1, tiles / 32));
         splits = least(most(fill, even), 128);
         splits = sums > kTickets ? 1 : least(splits, most(1, (uint32_t)(8192 / sums)));
-        if (a.sequences > 1 && a.sequences <= 64 && p.slots <= 512 && sums <= 2048 && tiles > 4) {
-            const uint32_t fill = most(2, 256 / a.kv_heads), safe = most(2, fill - least(fill, p.slots));
-            const uint32_t even = most(2, least(2048 / a.kv_heads, a.sequences * p.row_tiles * tiles / 32));
-            auto per = [](uint32_t n) { return (uint32_t)(((1ull << 32) + n - 1) / n); };
-            p.shares = Shares{most(fill, even), most(fill, even) + p.slots, p.slots, per(fill), per(safe), per(even)};
-        }
     } else {
         p.units = (uint32_t)sums;
         // two blocks a CU (a prompt of 512 rows in chunks of 8 tiles 30 us, of 4 tiles 33), or four of longer chunks
         splits = most(least(most(1, 512 / p.units), most(1, tiles / 8)), least(most(1, 1024 / p.units), most(1, tiles / 16)));
         splits = least(splits, 16);
+    }
+    const bool one = p.rows == 16;
+    const uint32_t row_tiles = one ? p.row_tiles : (uint32_t)(((uint64_t)tokens * a.group + 63) / 64);
+    // (of 64 rows where a sequence has few row tiles, and then for one round of blocks: eight sequences of 120 rows at 4,096
+    // positions 138 us by the longest and 113 so, of 48 rows at 700 to 8,192 91 and 83; many row tiles even themselves
+    // out: four sequences of 258 to 1,024 rows 327 and 332, but 848 and 803 in 512-wide heads, whose blocks have a CU each)
+    const bool uneven = row_tiles <= 4 || a.width == 512;
+    if (a.sequences > 1 && a.sequences <= 64 && p.slots <= 512 && sums <= (one ? 2048 : 512) && uneven && tiles > 4) {
+        const uint32_t few = one ? 4 : 8, some = one ? 32 : 16;
+        const uint32_t fill = most(2, (one || a.width == 512 ? 256 : 512) / a.kv_heads), safe = most(2, fill - least(fill, p.slots));
+        const uint32_t even = one ? most(2, least(2048 / a.kv_heads, a.sequences * row_tiles * tiles / some)) : fill;
+        auto per = [](uint32_t n) { return (uint32_t)(((1ull << 32) + n - 1) / n); };
+        p.shares = Shares{most(fill, even), most(fill, even) + p.slots, p.slots, per(fill), per(safe), per(even), few, some};
     }
     p.chunk = (tiles + splits - 1) / splits;
     p.splits = (tiles + p.chunk - 1) / p.chunk;
@@ -197,7 +205,7 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     // through to the memory side.  A prompt of 512 at 4,096 positions took 152 us joined by the last chunks, 111 apart.)
     p.join_apart = p.splits > 1 && (p.rows > 16 || p.splits * least(16, tokens * a.group) * row_bytes > 131072);
     p.part_bytes = p.splits > 1 ? (size_t)(sums * p.splits * p.rows * row_bytes) : 0;
-    if (p.shares.chunks) p.part_bytes = (size_t)((uint64_t)p.shares.chunks * a.kv_heads * 16 * row_bytes);
+    if (p.shares.chunks) p.part_bytes = (size_t)((uint64_t)p.shares.chunks * a.kv_heads * p.rows * row_bytes);
     return p;
 }
 

@@ -732,17 +732,17 @@ struct Share {
 
 // The sequence for whose lane find(start, span, its first chunk, the end of its chunks) is true, or false.
 template <typename F>
-__device__ __forceinline__ bool share(const PagedAttn& a, const Shares& sh, Share& o, F find) {
+__device__ __forceinline__ bool share(const PagedAttn& a, const Shares& sh, uint32_t R, Share& o, F find) {
     const uint32_t lane = threadIdx.x & 63, i = min(lane, a.b.sequences - 1);
     const uint32_t start = *gp(a.b.starts + i), stop = *gp(a.b.starts + i + 1), length = *gp(a.b.lengths + i);
     const Span s = span_of(start, stop, length, a.b);
-    const uint32_t r = lane < a.b.sequences ? (s.count * a.group + 15) / 16 : 0;
+    const uint32_t r = lane < a.b.sequences ? (s.count * a.group + R - 1) / R : 0;
     const uint32_t n = r ? tiles_of<32>(s.pos0, s.pos0 + (int32_t)s.count - 1, s.end, a.window, a.sinks).count : 0;
     const uint32_t row_tiles = __builtin_amdgcn_readlane(wave_prefix(r), 63), total = __builtin_amdgcn_readlane(wave_prefix(r * n), 63);
     if (row_tiles > sh.slots) return false;  // (starts that do not rise)
     uint32_t chunk, c, end;  // key tiles of the lane's chunks, chunks of a row tile, end of all of them
     auto deal = [&](uint32_t per_fill) {
-        chunk = share_chunk(share_of(total, per_fill, sh.per_even), n);
+        chunk = share_chunk(share_of(sh, total, per_fill), n);
         c = max(1u, quotient(n + chunk - 1, chunk));
         end = wave_prefix(r * c);
         return (uint32_t)__builtin_amdgcn_readlane(end, 63);
@@ -778,7 +778,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         h = blockIdx.x % a.kv_heads;
         const uint32_t b = blockIdx.x / a.kv_heads;
         Share o;
-        if (!share(a, shares, o, [&](uint32_t, const Span&, uint32_t first, uint32_t end) { return b >= first && b < end; })) return;
+        if (!share(a, shares, 16, o, [&](uint32_t, const Span&, uint32_t first, uint32_t end) { return b >= first && b < end; })) return;
         seq = o.seq;
         start = o.start;
         s = o.s;
@@ -1045,15 +1045,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
     if (shares.chunks) {
         Share o;  // (the last sequence whose slots begin at or before this one)
         const uint32_t at = slot / a.kv_heads;
-        if (!share(a, shares, o, [&](uint32_t start, const Span& s, uint32_t first, uint32_t end) {
-                const uint32_t base = s.first * a.group / 16 + (threadIdx.x & 63);
-                return end > first && at >= base && at < base + (s.count * a.group + 15) / 16;
+        if (!share(a, shares, R, o, [&](uint32_t, const Span& s, uint32_t first, uint32_t end) {
+                const uint32_t base = s.first * a.group / R + (threadIdx.x & 63);
+                return end > first && at >= base && at < base + (s.count * a.group + R - 1) / R;
             }))
             return;
         s = o.s;
         chunk = o.chunk;
         splits = kMaxParts;
-        tile = at - (o.start * a.group / 16 + o.seq);
+        tile = at - (o.s.first * a.group / R + o.seq);
         part = a.part + (size_t)(h * shares.chunks + o.first + tile * o.parts) * R * (W + 4);
     } else {
         slot_sequence(a, slot / a.kv_heads, R, tile, s);
@@ -1087,28 +1087,46 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
 
 template <int W, bool Q4>
 __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_many_kernel(PagedAttn a, uint32_t slots, uint32_t splits,
-                                                                                          uint32_t chunk) {
+                                                                                          uint32_t chunk, Shares shares) {
     constexpr int ST = W / 32, TV = W / 16, R = kManyRows;
     constexpr int E = W / 16 < 8 ? W / 16 : 8;  // channels of an octet
     constexpr int NK = Q4 ? (W + 255) / 256 : W / 64;  // a thread's pieces of K: blocks of 32 values, or octets
     constexpr int NV = (W + 255) / 256;                // and of V: four keys of an octet of channels
     __shared__ __align__(16) uint8_t lds[2][2][W * 64];  // [buffer][K, V]
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, g = lane >> 4;
-    // blocks b and b + 8 share an XCD: with heads times splits a multiple of 8, a head's row tiles share an L2
-    const uint32_t heads = a.kv_heads * splits;
-    uint32_t hs, slot;
-    if (heads % 8 == 0) {
-        hs = blockIdx.x / 8 / slots * 8 + blockIdx.x % 8;
-        slot = blockIdx.x / 8 % slots;
-    } else {
-        hs = blockIdx.x / slots;
-        slot = blockIdx.x % slots;
-    }
-    slot = slots - 1 - slot;  // (a sequence's last rows, which see the most keys, first)
-    const uint32_t h = hs % a.kv_heads, split = hs / a.kv_heads;
-    uint32_t rt;
+    uint32_t h, split, rt, seq;
     Span s;
-    const uint32_t seq = slot_sequence(a, slot, R, rt, s);
+    float* part = a.part;  // the chunk's partial sums
+    if (shares.chunks) {
+        h = blockIdx.x % a.kv_heads;
+        const uint32_t b = blockIdx.x / a.kv_heads;
+        Share o;
+        if (!share(a, shares, R, o, [&](uint32_t, const Span&, uint32_t first, uint32_t end) { return b >= first && b < end; })) return;
+        seq = o.seq;
+        s = o.s;
+        chunk = o.chunk;
+        splits = kMaxParts;
+        const uint32_t r = (s.count * a.group + R - 1) / R;
+        split = __builtin_amdgcn_readfirstlane(quotient(b - o.first, r));
+        rt = r - 1 - (b - o.first - split * r);  // (the last rows, which see the most keys, first)
+        part += (size_t)(h * shares.chunks + o.first + rt * o.parts + split) * R * (W + 4);
+    } else {
+        // blocks b and b + 8 share an XCD: with heads times splits a multiple of 8, a head's row tiles share an L2
+        const uint32_t heads = a.kv_heads * splits;
+        uint32_t hs, slot;
+        if (heads % 8 == 0) {
+            hs = blockIdx.x / 8 / slots * 8 + blockIdx.x % 8;
+            slot = blockIdx.x / 8 % slots;
+        } else {
+            hs = blockIdx.x / slots;
+            slot = blockIdx.x % slots;
+        }
+        slot = slots - 1 - slot;  // (a sequence's last rows, which see the most keys, first)
+        h = hs % a.kv_heads;
+        split = hs / a.kv_heads;
+        seq = slot_sequence(a, slot, R, rt, s);
+        part += ((size_t)(slot * a.kv_heads + h) * splits + split) * R * (W + 4);
+    }
     const uint32_t rows = s.count * a.group;
     if (rt * R >= rows) return;
     const uint32_t nr = min((uint32_t)R, rows - rt * R);
@@ -1449,7 +1467,6 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_ma
     if (idle) return;
 
     // rows to the output, or to the chunk's partial sums
-    float* part = a.part + ((size_t)(slot * a.kv_heads + h) * splits + split) * R * (W + 4);
     const float l = row_total(sm.l);
     float zero = l * 0.0f;
 #pragma unroll
@@ -1544,7 +1561,7 @@ hipError_t launch_paged_attention(const PagedAttn& a, uint32_t width, bool q4, c
                                p.units, p.shares.chunks ? kMaxParts : p.splits, p.shares.chunks ? p.slots : p.row_tiles, p.chunk,
                                p.join_apart, p.shares);
         } else {
-            hipLaunchKernelGGL((paged_many_kernel<W, Q4>), grid, block, 0, s, a, p.slots, p.splits, p.chunk);
+            hipLaunchKernelGGL((paged_many_kernel<W, Q4>), grid, block, 0, s, a, p.slots, p.splits, p.chunk, p.shares);
         }
         hipError_t e = hipGetLastError();
         if (e == hipSuccess && p.join_apart) {

@@ -319,7 +319,8 @@ def test_long_chunks_and_many_of_them(q4, new, hint):
 
 @pytest.mark.parametrize("q4,width", [(F16, 64), (Q4, 128), (Q4, 256), (F16, 512)])
 @pytest.mark.parametrize("new,lengths", [([1, 1], [2500, 30]), ([1, 0, 1, 1, 1], [200, 900, 0, 3000, 1400]),
-                                         ([6, 25, 1, 0, 9], [1000, 2600, 1, 50, 9]), ([1] * 64, [1 + 37 * i for i in range(64)])])
+                                         ([6, 25, 1, 0, 9], [1000, 2600, 1, 50, 9]),
+                                         ([50, 40, 1, 0, 64, 33], [1500, 3000, 2, 40, 64, 900]), ([1] * 64, [1 + 37 * i for i in range(64)])])
 def test_sequences_of_very_different_lengths(q4, width, new, lengths):
     """Chunks dealt out by the lengths there are: long beside short and empty ones, one and several row tiles, one more row
     behind the last sequence; with a window too."""
