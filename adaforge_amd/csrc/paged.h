@@ -117,7 +117,7 @@ AF_HD uint32_t longest_tiles(const AttnShape& a, uint32_t tokens) {
 
 constexpr uint32_t kManyRows = 64;
 
-// Chunks shared out by the work there is, not by the longest sequence: 2 to 64 sequences, whose key tiles every block adds up
+// Chunks shared out by the work there is, not by the longest sequence: up to 64 sequences, whose key tiles every block adds up
 // for itself (a lane a sequence).  A KV head's chunks take `chunks` blocks at most (0: shared
 // out by the hints), of which those that fill the chip or even out what is left are `most`, and one a row tile
 // (`slots`).  32 conversations of 1 to 8,192 positions took 229 us by the longest and take 205 so, eight of 512-wide
@@ -161,12 +161,14 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     const uint64_t pairs = (uint64_t)a.sequences * a.kv_heads;  // (at most 2^22: checked by the call)
     const uint32_t tiles = longest_tiles(a, tokens);
     p.row_tiles = (uint32_t)(((uint64_t)tokens * a.group + 15) / 16);
-    // Up to four row tiles of 16 read K and V once each (from an L2), more share them through LDS, 64 rows at a time.  Eight
-    // sequences of 4,096 positions, 256-wide 4-bit heads: three tiles 72 us, by 64 rows 87, four 89 and 98, five 110 and
-    // 111, eight 168 and 138.  256-wide fp16 rows, which need the most from the L2, share from three tiles on once there
-    // are key tiles enough to fill the chip: three sequences of 4,096 positions 63 us and 47, eight of 1,000 34 and 37.
-    const bool heavy = !a.q4 && a.width == 256 && pairs * tiles > 2048;
-    p.rows = p.row_tiles > (heavy ? 2u : 4u) ? kManyRows : 16;
+    // Row tiles of 16 read K and V once each, through an L2; tiles of 64 rows share them through LDS, which pays as soon as
+    // what is read fills the chip.  With fewer key tiles, from five row tiles on: eight sequences of 300 positions, three
+    // row tiles of 256-wide fp16 heads 20 us, by 64 rows 23; of 1,000 in 128-wide heads 21 and 29; 80 rows at 300 22 and 18.
+    // With more, from three on: eight of 4,096, three row tiles of 256-wide 4-bit heads 74 and 63, 16 of up to 16,000 in
+    // 512-wide heads, four row tiles 148 and 100, fp16 231 and 99.  From two on where a row tile reads most: 512 wide 149 and
+    // 77, 4 bits 97 and 79, 256-wide fp16 102 and 77, 128-wide 56 and 46 (but 4 bits 45 and 51, 64-wide 31 and 34).
+    const uint32_t apart = pairs * tiles <= 2048 ? 4 : a.width == 512 || (!a.q4 && a.width >= 128) ? 1 : 2;
+    p.rows = p.row_tiles > apart ? kManyRows : 16;
     p.slots = row_slots(a, p.rows);
     if (p.row_tiles * pairs > 1u << 22) p.row_tiles = most(1, (uint32_t)((1u << 22) / pairs));
     const uint64_t sums = (uint64_t)p.slots * a.kv_heads;
@@ -185,21 +187,21 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
         splits = most(least(most(1, 512 / p.units), most(1, tiles / 8)), least(most(1, 1024 / p.units), most(1, tiles / 16)));
         splits = least(splits, 16);
     }
+    p.chunk = (tiles + splits - 1) / splits;
+    p.splits = (tiles + p.chunk - 1) / p.chunk;
     const bool one = p.rows == 16;
     const uint32_t row_tiles = one ? p.row_tiles : (uint32_t)(((uint64_t)tokens * a.group + 63) / 64);
     // (of 64 rows where a sequence has few row tiles, and then for one round of blocks: eight sequences of 120 rows at 4,096
     // positions 138 us by the longest and 113 so, of 48 rows at 700 to 8,192 91 and 83; many row tiles even themselves
     // out: four sequences of 258 to 1,024 rows 327 and 332, but 848 and 803 in 512-wide heads, whose blocks have a CU each)
-    const bool uneven = row_tiles <= 4 || a.width == 512;
-    if (a.sequences > 1 && a.sequences <= 64 && p.slots <= 512 && sums <= (one ? 2048 : 512) && uneven && tiles > 4) {
+    const bool uneven = one ? a.sequences > 1 && tiles > 4 : p.splits > 1 && (row_tiles <= 4 || a.width == 512);
+    if (uneven && a.sequences <= 64 && p.slots <= 512 && sums <= (one ? 2048 : 512)) {
         const uint32_t few = one ? 4 : 8, some = one ? 32 : 16;
         const uint32_t fill = most(2, (one || a.width == 512 ? 256 : 512) / a.kv_heads), safe = most(2, fill - least(fill, p.slots));
         const uint32_t even = one ? most(2, least(2048 / a.kv_heads, a.sequences * row_tiles * tiles / some)) : fill;
         auto per = [](uint32_t n) { return (uint32_t)(((1ull << 32) + n - 1) / n); };
         p.shares = Shares{most(fill, even), most(fill, even) + p.slots, p.slots, per(fill), per(safe), per(even), few, some};
     }
-    p.chunk = (tiles + splits - 1) / splits;
-    p.splits = (tiles + p.chunk - 1) / p.chunk;
     const uint64_t row_bytes = (uint64_t)(a.width + 4) * 4;
     // (many partial sums are stored, and joined, faster by many blocks of another launch: its partial sums need not go
     // through to the memory side.  A prompt of 512 at 4,096 positions took 152 us joined by the last chunks, 111 apart.)

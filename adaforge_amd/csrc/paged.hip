@@ -346,7 +346,7 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
     }
 }
 
-// ---- attention of few rows: single tokens and short drafts ---------------------------------------------
+// ---- attention of few rows: single tokens, and short drafts over few keys --------------------------------
 //
 // Rows are the (token, query head) pairs that share a KV head: row i of a sequence is token i / group, head i % group.
 // A block takes 16 of them against a chunk of the sequence's key tiles, its four waves tile by tile in turn; the
@@ -1070,7 +1070,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttn a, uint32_t s
     join_parts<W, S>(a, part, parts, R, c0, min(nr, c0 + 4 / S), tile * R, s.first, h);
 }
 
-// ---- attention of many rows: prompts and further turns --------------------------------------------------
+// ---- attention of many rows: drafts, prompts and further turns -------------------------------------------
 //
 // Row tiles of 64 rows: a wave holds 16 of them from scores to output, their queries and sums in registers, and
 // the block's four waves share K and V through LDS, 32 keys at a time in two buffers: while one tile is used, the next

@@ -328,15 +328,15 @@ def test_sequences_of_very_different_lengths(q4, width, new, lengths):
     kv = kp.values(), vp.values()
     for window, sinks in ((0, 0), (700, 40)):
         want = R.attention(b, *kv, q, 1, 1 / np.sqrt(width), window, sinks)
-        for longest in ((max(new), max(lengths)), (1, 300)):
+        for longest in ((max(new), max(lengths)), (1, 300), (max(new), 300), (max(new), 450), (max(new), 1 << 24)):
             got, _ = run_attention(b, kp, vp, q, 1, window, sinks, longest)
             R.check_attention(got, want, width, 2.0)
             assert (got[sum(new):] == -7).all()
 
 
-@pytest.mark.parametrize("q4,width", [(F16, 256), (F16, 128), (Q4, 256)])
-@pytest.mark.parametrize("new", [[24, 17, 1, 20, 24, 9, 3, 23], [29, 32, 0, 31, 8, 25, 30, 2]])
-def test_three_and_four_row_tiles_over_many_keys(q4, width, new):
+@pytest.mark.parametrize("q4,width", [(F16, 256), (F16, 128), (Q4, 256), (Q4, 512), (F16, 64)])
+@pytest.mark.parametrize("new", [[24, 17, 1, 20, 24, 9, 3, 23], [16, 9, 1, 10, 0, 2, 12, 16], [29, 32, 0, 31, 8, 25, 30, 2]])
+def test_a_few_row_tiles_over_many_keys(q4, width, new):
     """Row tiles of 16 and of 64 rows, whichever the launch takes for these types and widths."""
     lengths = [1100, 40, 700, 1099, 24, 513, 3, 800]
     lengths = [max(n, m) for n, m in zip(lengths, new)]
