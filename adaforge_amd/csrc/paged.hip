@@ -769,7 +769,12 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                                                                           Shares shares) {
     constexpr int ST = W / 32, TV = W / 16, HALFROWS = 8;
     using V = VHalf<W, Q4, NT>;
-    __shared__ __align__(16) uint8_t lds[W * 128];  // the queries' operands; at the end eight rows of each wave's sums
+    // At the end eight rows of each wave's sums lie in LDS.  512 wide, with four floats behind every 4 E of them and rows 16
+    // floats past a multiple of 64, so that a write's lanes (8 rows, 4 places 4 E apart) take different banks: eight
+    // sequences of up to 32,768 positions 45.5 -> 43.8 us; 256 wide the addresses cost registers (52 -> 54 us).
+    constexpr int SKEW = 4 * V::E, ROW = W == 512 ? (W + W / V::E - 16 + 63) / 64 * 64 + 16 : W;
+    auto skewed = [](uint32_t x) { return W == 512 ? x + x / SKEW * 4 : x; };
+    __shared__ __align__(16) uint8_t lds[4 * HALFROWS * ROW * 4];  // (the queries' operands before: 64 W bytes)
     __shared__ float wm[4][16], wl[4][16];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, g = lane >> 4;
     uint32_t h, seq, tile0, split, start, part0 = 0;  // part0: of the row tile's chunks, in shares
@@ -956,7 +961,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
         odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;
 
         // the waves' sums meet in LDS, eight rows at a time
-        float* sums = reinterpret_cast<float*>(lds);  // [wave][row of 8][W]
+        float* sums = reinterpret_cast<float*>(lds);  // [wave][row of 8][ROW]
         const uint32_t slot = (start * a.group / 16 + seq + rt) * a.kv_heads + h;
         float* parts0 = a.part + (shares.chunks ? (size_t)part0 : (size_t)slot * splits) * 16 * (W + 4);
         float* part = parts0 + (size_t)split * 16 * (W + 4);
@@ -970,12 +975,12 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
             if (r0) __syncthreads();
             const uint32_t r = m - r0;
             if (r < HALFROWS && m < nr) {
-                float* dst = sums + (wave * HALFROWS + r) * W;
+                float* dst = sums + (wave * HALFROWS + r) * ROW;
 #pragma unroll
                 for (int t = 0; t < TV; t += 4)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        *reinterpret_cast<f4*>(dst + 16 * V::E * (t / V::E) + V::E * (4 * g + e) + t % V::E) =
+                        *reinterpret_cast<f4*>(dst + (4 * (t / V::E) + g) * (W == 512 ? SKEW + 4 : SKEW) + V::E * e + t % V::E) =
                             f4{acc[t][e], acc[t + 1][e], acc[t + 2][e], acc[t + 3][e]};
             }
             for (uint32_t bad = (uint32_t)(odd >> r0) & 0xFF; bad; bad &= bad - 1) {
@@ -990,7 +995,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                 plain_row<W, Q4, 32>(a, keys, t0, t1, 4, seq, h, s.pos0 + (int32_t)(row / a.group), s.end, q, o, pm, pl2);
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int e = 0; e < E; ++e) sums[(wave * HALFROWS + c - r0) * W + E * lane + e] = o[e];
+                for (int e = 0; e < E; ++e) sums[(wave * HALFROWS + c - r0) * ROW + skewed(E * lane + e)] = o[e];
                 if (lane == 0) {
                     wm[wave][c] = pm * kLog2e + kProbBits;  // (its sums lack the others' factor)
                     wl[wave][c] = pl2;
@@ -1007,7 +1012,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                 for (int w = 0; w < 4; ++w) {
                     const float f = wm[w][r0 + c] == -INFINITY && wl[w][r0 + c] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(wm[w][r0 + c] - M);
                     L = fmaf(f, wl[w][r0 + c], L);
-                    if (f != 0.0f) o += f * *reinterpret_cast<const f4*>(sums + (w * HALFROWS + c) * W + x);
+                    if (f != 0.0f) o += f * *reinterpret_cast<const f4*>(sums + (w * HALFROWS + c) * ROW + skewed(x));
                 }
                 if (parts == 1) {
                     float* out = a.out + (size_t)(s.first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;

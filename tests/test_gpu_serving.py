@@ -461,6 +461,28 @@ def test_an_infinity_reaches_only_the_positions_that_see_it(new, before, where, 
     assert np.linalg.norm(g - w) <= 2 * R.attention_bound(64, 2.0) * np.linalg.norm(w)
 
 
+@pytest.mark.parametrize("q4,width", [(F16, 128), (Q4, 128), (F16, 256), (Q4, 256), (F16, 512), (Q4, 512)])
+@pytest.mark.parametrize("new", [[3, 1], [40, 9]])
+def test_not_a_number_among_the_keys_of_every_width(q4, width, new):
+    """One key that is no number, seen by some rows of a tile and not by others: those are as without it."""
+    rng, b, kp, vp, q = make_attention(("nan", int(q4), width, new[0]), q4, width, 16, 4, 2, new, [700, 90])
+    clean = R.attention(b, kp.values(), vp.values(), q, 2, 1 / np.sqrt(width))
+    at = b.place(0, 700 - new[0] // 2 - 1)
+    if q4:
+        codes, scales = kp.planes()
+        scales[at[0], 1, at[1], 1] = np.nan
+        kp._join(codes, scales)
+    else:
+        kp.planes()[0][at[0], 1, at[1], 7] = np.nan
+    got, _ = run_attention(b, kp, vp, q, 2)
+    seen = new[0] - new[0] // 2 - 1  # the first row whose position is the key's
+    assert np.isnan(got[seen:new[0], 2:]).all()
+    want = clean.copy()
+    want[seen:new[0], 2:] = 0
+    got[seen:new[0], 2:] = 0
+    R.check_attention(got, want, width, 2.0)
+
+
 @pytest.mark.parametrize("q4", [F16, Q4])
 @pytest.mark.parametrize("n", [1, 34])
 def test_large_and_small_queries(q4, n):
