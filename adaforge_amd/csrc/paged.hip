@@ -354,7 +354,7 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
 // data with a running maximum and sum).  Bound by reading K and V once: one token at 32,768 positions (8 heads of 256,
 // fp16, 268 MB) 50.6 us = 5.3 TB/s, 32 of 1 to 8,192 positions 204 us = 5.3 TB/s; 4-bit rows by unpacking them (13
 // instructions a word of eight) and by the waits between dependent steps: 64 windows of 1,024 41.8 us = 3.6 TB/s, eight
-// 512-wide heads of up to 32,768 positions (a block a CU) 38 us and 7 the join; short contexts by the chain of the
+// 512-wide heads of up to 32,768 positions (a block a CU) 35 us and 7 the join; short contexts by the chain of the
 // sequence's place, the page numbers, K, V, the ticket and the join: one token at 512 positions 10.6 us.
 //
 // Products are taken transposed on the fp16 matrix cores, S^T = K Q^T and O^T = V^T P^T (16 keys or channels by 16
