@@ -166,8 +166,9 @@ AF_HD AttnPlan attn_plan(const AttnShape& a) {
     // row tiles of 256-wide fp16 heads 20 us, by 64 rows 23; of 1,000 in 128-wide heads 21 and 29; 80 rows at 300 22 and 18.
     // With more, from three on: eight of 4,096, three row tiles of 256-wide 4-bit heads 74 and 63, 16 of up to 16,000 in
     // 512-wide heads, four row tiles 148 and 100, fp16 231 and 99.  From two on where a row tile reads most: 512 wide 149 and
-    // 77, 4 bits 97 and 79, 256-wide fp16 102 and 77, 128-wide 56 and 46 (but 4 bits 45 and 51, 64-wide 31 and 34).
-    const uint32_t apart = pairs * tiles <= 2048 ? 4 : a.width == 512 || (!a.q4 && a.width >= 128) ? 1 : 2;
+    // 77, 4 bits 97 and 79, 256-wide fp16 102 and 77, 128-wide 56 and 46 (but 4 bits 45 and 51, 64-wide 31 and 34).  64-wide
+    // 4-bit heads read the least: 100 of 400 to 4,000, three row tiles 149 and 207.
+    const uint32_t apart = pairs * tiles <= 2048 || (a.q4 && a.width == 64) ? 4 : a.width == 512 || (!a.q4 && a.width >= 128) ? 1 : 2;
     p.rows = p.row_tiles > apart ? kManyRows : 16;
     p.slots = row_slots(a, p.rows);
     if (p.row_tiles * pairs > 1u << 22) p.row_tiles = most(1, (uint32_t)((1u << 22) / pairs));
