@@ -286,16 +286,22 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const uint8_t* k_pages, co
     }
 }
 
+constexpr float kLog2e = 1.44269504088896340736f, kLog2eLow = 1.92596299112661746887e-8f;  // log2(e), and what its float lacks
+
 // ---- attention, key by key ----------------------------------------------------------------------------
 
 // Softmax attention of one query by one wave, key by key in fp32 over key tiles t0, t0 + step, .. below t1 of T keys:
 // values are read only where the query sees them.  What the products below fall back to where a sum of theirs is
 // not finite: there an infinite cached value meets halves of a pair that are zero or of the other sign, also
-// of keys that the row does not see.  Lane: channels E lane .. E lane + E - 1 (E = W / 64).
+// of keys that the row does not see; and where scores are so large that fp32 holds them to no less than parts of a unit (far_off).
+// Lane: channels E lane .. E lane + E - 1 (E = W / 64).  The sums are left as the products hold theirs, times 2^-m for a whole m (the
+// nearest to the maximum in base 2, whose remainder goes into them: maxima of 2^30, held to 128, would else join
+// as equals).
 template <int W, bool Q4, uint32_t T>
 __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles, uint32_t t0, uint32_t t1, uint32_t step,
                                           uint32_t seq, uint32_t h, int32_t pos, uint32_t end, const float (&q)[W / 64],
                                           float (&acc)[W / 64], float& m, float& l) {
+#pragma clang fp contract(off)  // (a score less the maximum: both rounded, or the largest key's weight is not 1)
     constexpr int E = W / 64;
     const uint32_t lane = threadIdx.x & 63, tokens = 1u << a.b.page_shift;
     const uint32_t bytes = page_part_bytes(Q4, tokens, W);
@@ -333,16 +339,28 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
             for (int e = 0; e < E; ++e) d = fmaf(q[e], v[e], d);
             const float s = wave_sum(d) * a.scale, mn = fmaxf(m, s);
             const float p = s == -INFINITY ? 0.0f : expf(s - mn), al = mn == -INFINITY ? 1.0f : expf(m - mn);
-            l = fmaf(l, al, p);
+            // (the weights, which lanes have alike, by lanes: thousands of like terms in one sum would all round the same way)
+            l = fmaf(l, al, lane == (j & 63) ? p : 0.0f);
             row(a.v_pages + off, slot, v);
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] = p > 0.0f || p != p ? fmaf(p, v[e], acc[e] * al) : acc[e] * al;
             m = mn;
-            if (l != l) {  // every output is a NaN
+            if (p != p) {  // every output is a NaN
                 m = 0.0f;
+                l = p;
                 return;
             }
         }
+    }
+    l = wave_sum(l);
+    if (m > -INFINITY) {
+        const float whole = rintf(m * kLog2e), rest = fmaf(m, kLog2e, -whole) + m * kLog2eLow;
+        // (a remainder past 60: from 2^30 on, where unequal maxima are further apart than 2^60 in their weights anyway)
+        const float f = __builtin_amdgcn_exp2f(fminf(fmaxf(rest, -60.0f), 60.0f));
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= f;
+        l *= f;
+        m = whole;
     }
 }
 
@@ -370,7 +388,6 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
 
 constexpr int kPartSC1 = 16;      // buffer access policy sc1: through to (or from) the memory side
 constexpr int kWaitVm0 = 0x0F70;  // s_waitcnt vmcnt(0), expcnt and lgkmcnt unconstrained
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kProbBits = 8.0f;  // weights are held times 2^8 ..
 constexpr float kRise = 7.0f;      // .. against a maximum that may have risen by this since: below fp16's 2^16
 
@@ -617,6 +634,10 @@ struct Softmax {
 #pragma unroll
         for (int k = 0; k < 8; ++k) slice(k, s, qs, w);
     }
+
+    // Whether the maximum is so far from 0 that its own rounding (half of 2^-2 at 2^21), and that of off, would move the weights out
+    // of fp16's range: the largest past 2^16, or all of them below 2^-24 while l has them.
+    __device__ __forceinline__ bool far_off() const { return m > -INFINITY && fabsf(m) > 0x1p21f; }
 };
 
 // The chunks of a row tile of `tiles` key tiles: chunk tiles each, or more where they would be over `splits`.
@@ -951,13 +972,17 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
             }
             if (more) load_v(t + 4, here);
         }
+        // (places made again from the thread's number: kept over the loop they spill)
+        uint32_t me = threadIdx.x;
+        asm volatile("" : "+v"(me));
+        const uint32_t tid = me, lane = me & 63, m = me & 15, g = lane >> 4;
         const float lrun = row_total(sm.l);
 
-        // columns whose sums are not finite
+        // columns whose sums are not finite, or whose scores are far off
         float zero = lrun * 0.0f;
 #pragma unroll
         for (int t = 0; t < TV; ++t) zero += (acc[t][0] + acc[t][1] + acc[t][2] + acc[t][3]) * 0.0f;
-        uint64_t odd = __ballot(!(zero == 0.0f));
+        uint64_t odd = __ballot(!(zero == 0.0f) | sm.far_off());
         odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;
 
         // the waves' sums meet in LDS, eight rows at a time
@@ -997,7 +1022,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
 #pragma unroll
                 for (int e = 0; e < E; ++e) sums[(wave * HALFROWS + c - r0) * ROW + skewed(E * lane + e)] = o[e];
                 if (lane == 0) {
-                    wm[wave][c] = pm * kLog2e + kProbBits;  // (its sums lack the others' factor)
+                    wm[wave][c] = pm + kProbBits;  // (its sums lack the others' factor)
                     wl[wave][c] = pl2;
                 }
             }
@@ -1476,8 +1501,8 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_ma
     float zero = l * 0.0f;
 #pragma unroll
     for (int t = 0; t < TV; ++t) zero += (acc[t][0] + acc[t][1] + acc[t][2] + acc[t][3]) * 0.0f;
-    uint64_t odd = __ballot(!(zero == 0.0f));
-    odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;  // columns whose sums are not finite
+    uint64_t odd = __ballot(!(zero == 0.0f) | sm.far_off());
+    odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;  // columns whose sums are not finite, or whose scores are far off
     if (row < rows && !(odd >> m & 1)) {
         float* out = a.out + (size_t)(s.first + row / a.group) * a.out_stride + (size_t)(h * a.group + row % a.group) * W;
         float* dst = parts == 1 ? out : part + (row - rt * R) * (W + 4);
@@ -1507,7 +1532,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_ma
 #pragma unroll
         for (int e = 0; e < EL; ++e) dst[e] = parts > 1 ? o[e] : pl == 0.0f ? 0.0f : o[e] / pl;
         if (parts > 1 && lane == 0) {  // (without the others' factor)
-            part[(r - rt * R) * (W + 4) + W] = pm * kLog2e + kProbBits;
+            part[(r - rt * R) * (W + 4) + W] = pm + kProbBits;
             part[(r - rt * R) * (W + 4) + W + 1] = pl;
         }
     }
