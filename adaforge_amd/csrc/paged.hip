@@ -384,12 +384,10 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
 // base address is scalar and every load adds a constant per lane.
 //
 // fp32 rows enter as fp16 pairs hi + lo (22 bits and more): queries scaled by a power of two to below 32,
-// weights times 2^8, which the exponent takes in (Softmax).
+// weights by one that the exponent takes in (Softmax).
 
 constexpr int kPartSC1 = 16;      // buffer access policy sc1: through to (or from) the memory side
 constexpr int kWaitVm0 = 0x0F70;  // s_waitcnt vmcnt(0), expcnt and lgkmcnt unconstrained
-constexpr float kProbBits = 8.0f;  // weights are held times 2^8 ..
-constexpr float kRise = 7.0f;      // .. against a maximum that may have risen by this since: below fp16's 2^16
 
 // The first key that a query at position p sees, apart from the first tokens.
 __device__ __forceinline__ int32_t first_seen(int32_t p, uint32_t window) {
@@ -591,24 +589,41 @@ struct VHalf {
     }
 };
 
-// The column's running softmax (base 2): weights 2^(score - m + kProbBits), m a maximum of the scores so far that lags
-// behind by at most kRise, so that the sums are rescaled for the first tiles and then hardly ever.
+// The column's running softmax (base 2): weights 2^(score - m), as fp16 pairs, which have 22 bits from 2^-3 up to 2^16.  So m, a whole
+// number, follows the tiles: where a tile's largest weight would be above 2^kHigh or below 1, m moves and the sums are rescaled
+// (exactly).  It moves to make that weight about 2^kSet, which later tiles seldom leave; or 2^kAlone where one lane's eight keys stand
+// kApart above another's: a key that may have most of the weight for itself, beside which the others' bits matter if its value
+// is small.  And it moves down again behind such a key: first tokens that draw nearly all of the weight and add nothing leave an
+// output of the others' weights.  2,500 keys, the first with a share of 0.9995 and a value of zero: 5e-7 of the output wrong in
+// one chunk, 4e-6 to 2e-4 against one maximum that only rises.  But m stays within 2^kBack of its highest, so that the sums do not
+// overflow: weights that lose bits by that are below 2^-68 of the sum.
+constexpr float kSet = 8.0f, kAlone = 14.0f, kApart = 8.0f, kHigh = 15.5f, kBack = 60.0f;
+constexpr float kNone = -3.402823466e38f;  // m of a column that has seen nothing
+
 struct Softmax {
-    float m = -INFINITY, l = 0.0f, off = 0.0f;  // l: the sum over this lane's keys; off = kProbBits - m
+    float m = kNone, top = kNone, l = 0.0f;  // top: the highest m; l: the sum over this lane's keys
 
     // Takes in the lane's scores of eight keys (times qs; -inf: not seen): scale(f) gets the factor of the sums so far
     // where it is not 1 (lanes of a column agree).
     template <typename F>
-    __device__ __forceinline__ void rise(const f4 (&s)[2], float qs, F scale) {
+    __device__ __forceinline__ void follow(const f4 (&s)[2], float qs, F scale) {
         const float mine = qs * fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        if (__ballot(mine > m + kRise)) {
-            const float mx = fmaxf(m, lanes4_max(mine));
-            const float al = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
-            m = mx;
-            off = mx == -INFINITY ? 0.0f : kProbBits - mx;
-            l *= al;
-            scale(al);
+        if (__ballot(!(fabsf(mine - m - 0.5f * kHigh) <= 0.5f * kHigh))) {
+            const uint64_t low = __ballot(!(mine - m >= 0.0f)), lows = low & low >> 32;  // (a column is low where its four lanes are)
+            if (!(__ballot(mine - m > kHigh) | (lows & lows >> 16 & 0xFFFF))) return;
+            const float mx = lanes4_max(mine), over = mx - m;
+            const bool alone = mx + lanes4_max(mine > -INFINITY ? -mine : -INFINITY) > kApart;
+            const float to = over > kHigh || (over < 0.0f && mx > -INFINITY) ? fmaxf(rintf(mx - (alone ? kAlone : kSet)), top - kBack) : m;
+            if (__ballot(to != m)) {
+                const float al = __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                top = fmaxf(top, to);
+                if (__ballot(l != 0.0f)) {  // (not for a wave's first tile)
+                    l *= al;
+                    scale(al);
+                }
+            }
         }
     }
 
@@ -622,7 +637,7 @@ struct Softmax {
     __device__ __forceinline__ void slice(int k, const f4 (&s)[2], float qs, Weights& w) {
         if (k < 4) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) w.p[2 * k + e] = __builtin_amdgcn_exp2f(fmaf(s[k / 2][k % 2 * 2 + e], qs, off));
+            for (int e = 0; e < 2; ++e) w.p[2 * k + e] = __builtin_amdgcn_exp2f(fmaf(s[k / 2][k % 2 * 2 + e], qs, -m));
         } else {
             k -= 4;
             w.hi[k] = pack_f16(w.p[2 * k], w.p[2 * k + 1]);
@@ -635,9 +650,9 @@ struct Softmax {
         for (int k = 0; k < 8; ++k) slice(k, s, qs, w);
     }
 
-    // Whether the maximum is so far from 0 that its own rounding (half of 2^-2 at 2^21), and that of off, would move the weights out
-    // of fp16's range: the largest past 2^16, or all of them below 2^-24 while l has them.
-    __device__ __forceinline__ bool far_off() const { return m > -INFINITY && fabsf(m) > 0x1p21f; }
+    // Whether m is so far from 0 that its distance from scores is rounded (by 2^-3 at 2^21) and weights may leave fp16's range: above
+    // 2^16, or all of them below 2^-24 while l has them.
+    __device__ __forceinline__ bool far_off() const { return m > kNone && fabsf(m) > 0x1p21f; }
 };
 
 // The chunks of a row tile of `tiles` key tiles: chunk tiles each, or more where they would be over `splits`.
@@ -948,7 +963,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                         if (!(in & (j <= hi_all) & ((j >= lo_all) | (j < first)))) here.v[i].clear(e);
                     }
             }
-            sm.rise(sv, qs, [&](float f) {
+            sm.follow(sv, qs, [&](float f) {
 #pragma unroll
                 for (int i = 0; i < TV; ++i) acc[i] *= f;
             });
@@ -1022,7 +1037,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
 #pragma unroll
                 for (int e = 0; e < E; ++e) sums[(wave * HALFROWS + c - r0) * ROW + skewed(E * lane + e)] = o[e];
                 if (lane == 0) {
-                    wm[wave][c] = pm + kProbBits;  // (its sums lack the others' factor)
+                    wm[wave][c] = pm;
                     wl[wave][c] = pl2;
                 }
             }
@@ -1378,7 +1393,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_ma
                     const int32_t j = now.j0 + 16 * i + 4 * (int32_t)g + e;
                     sv[i][e] = (now.ok >> i & 1) & (j <= hi_m) & ((j >= lo_m) | (j < first)) ? sv[i][e] : -INFINITY;
                 }
-        sm.rise(sv, qs, [&](float f) {
+        sm.follow(sv, qs, [&](float f) {
 #pragma unroll
             for (int v = 0; v < TV; ++v) acc[v] *= f;
         });
@@ -1531,8 +1546,8 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_ma
         float* dst = parts == 1 ? a.out + token * a.out_stride + at : part + (r - rt * R) * (W + 4) + EL * lane;
 #pragma unroll
         for (int e = 0; e < EL; ++e) dst[e] = parts > 1 ? o[e] : pl == 0.0f ? 0.0f : o[e] / pl;
-        if (parts > 1 && lane == 0) {  // (without the others' factor)
-            part[(r - rt * R) * (W + 4) + W] = pm + kProbBits;
+        if (parts > 1 && lane == 0) {
+            part[(r - rt * R) * (W + 4) + W] = pm;
             part[(r - rt * R) * (W + 4) + W + 1] = pl;
         }
     }

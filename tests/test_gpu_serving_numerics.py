@@ -17,9 +17,15 @@ def norm_error(got, want):
 # ---- large scores -------------------------------------------------------------------------------------
 #
 # Where a key takes everything the answer is its value.  What the arithmetic may add: the weight as two fp16 halves (2^-23 of it),
-# its product and sum (2^-24 each), the division and the factor of a join (2^-23 together): below 2^-21.
+# its products and their sum (2^-23: the matrix unit cuts bits off before it rounds), the division and the factor of a join (2^-23
+# together): below 2^-21.  A value below fp16's normal numbers enters the unit with the exponent of 2^-14, and bits are cut off
+# there (a b + c measured: wrong by 2^-23 of it from 2^-14 up, 2^-22 at 2^-16, 2^-18 at 2^-20, 2^-14 at 2^-24).
 
 LARGE = [2.0 ** 20, 2.0 ** 27, 2.0 ** 29, 2.0 ** 32]
+
+
+def is_value(got, want):
+    return (np.abs(got - want) <= 2.0 ** -21 * np.maximum(np.abs(want), 2.0 ** -14)).all()
 
 
 @pytest.mark.parametrize("large", LARGE)
@@ -37,7 +43,7 @@ def test_one_visible_key_of_any_score(new, q4, width, large):
             q[row, h] *= large * rng.uniform(0.5, 2) / abs(score)
             want[row, h] = v[pg, h // 2, slot]
     got, _ = run_attention(b, kp, vp, q, 2, window=1)
-    assert (np.abs(got - want) <= 2.0 ** -21 * np.abs(want)).all(), np.abs(got - want).max()
+    assert is_value(got, want), np.abs(got - want).max()
 
 
 @pytest.mark.parametrize("large", LARGE)
@@ -61,7 +67,7 @@ def test_one_key_far_above_the_others(new, q4, width, large):
         want = vp.values()[pg, 0, slot].astype(np.float64)
         for hint in ((max(new), n), (max(new), 1)):
             got, _ = run_attention(b, kp, vp, q, 1, longest=hint)
-            assert (np.abs(got[:new[0]] - want) <= 2.0 ** -21 * np.abs(want)).all(), (at, hint, np.abs(got[:new[0]] - want).max())
+            assert is_value(got[:new[0]], want), (at, hint, np.abs(got[:new[0]] - want).max())
 
 
 @pytest.mark.parametrize("power", [10, 18, 20, 21, 22, 23, 24, 26, 29])
@@ -87,3 +93,75 @@ def test_differences_of_large_scores(new, sign, power):
         # half an ulp, 2^-24 at most, so that n of them add up to 2^-24 / sqrt(3) sqrt(n / 2); three times that.
         bound = 2.0 ** -19 + 3 * 2.0 ** -24 / np.sqrt(3) * np.sqrt(n / 2)
         assert norm_error(got, want) <= bound, (hint, norm_error(got, want), bound)
+
+
+# ---- one key that takes nearly all of the weight -------------------------------------------------------
+
+def sunk(key, q4, width, new, n, share, rng_new=None):
+    """Sequence 0 of n positions whose first key, of value zero, takes about `share` of every row's weight: the output is what the
+    others add.  The first key's score is one product, s0 for every row; the others' are about N(0, 1)."""
+    rng, b, kp, vp, q = make_attention(key, q4, width, 64, 2, 1, new, [n, 60], spread=1.0)
+    keys, values = f32(rng, *kp.values().shape), f32(rng, *vp.values().shape)
+    keys[..., 0] = 0
+    pg, slot = b.place(0, 0)
+    keys[pg, :, slot] = 0
+    keys[pg, :, slot, 0] = 8
+    values[pg, :, slot] = 0
+    kp.set(keys)
+    vp.set(values)
+    s0 = np.log(n * np.exp(0.5) * share / (1 - share))
+    q[..., 0] = s0 * np.sqrt(width) / 8
+    return b, kp, vp, q, s0
+
+
+@pytest.mark.parametrize("share", [0.5, 0.97, 0.996, 0.9995, 0.9999])
+@pytest.mark.parametrize("q4,width", [(F16, 64), (Q4, 64), (F16, 256), (Q4, 128), (F16, 512)])
+@pytest.mark.parametrize("new", [FEW, MANY])
+def test_a_first_key_that_takes_nearly_all_of_the_weight(new, q4, width, share):
+    """First tokens that draw the attention and add nothing: what remains of the output keeps its digits.
+
+    Bound: that of 32-bit scores and sums, the first key's score once more for every row (2^-24 s0 and as much for its exponential's
+    argument), and for the keys of its tile, whose weights are held to 2^-38 of the largest there (one 78th of the keys,
+    their errors uniform): 3 times 2^-38 / sqrt(3) over their mean weight."""
+    n = 2500
+    b, kp, vp, q, s0 = sunk(("sink", int(q4), width, new[0]), q4, width, new, n, share)
+    want = R.attention(b, kp.values(), vp.values(), q, 1, 1 / np.sqrt(width))
+    mean = (1 - share) / n / share
+    bound = R.attention_bound(width, 1.0) + 2.0 ** -23 * s0 + 3 * 2.0 ** -38 / np.sqrt(3) / mean * np.sqrt(32 / n)
+    for hint in ((max(new), n), (max(new), 1)):
+        got, _ = run_attention(b, kp, vp, q, 1, longest=hint)
+        rows = slice(0, new[0])
+        assert norm_error(got[rows], want[rows]) <= bound, (hint, norm_error(got[rows], want[rows]), bound)
+
+
+@pytest.mark.parametrize("new", [FEW, MANY])
+@pytest.mark.parametrize("q4", [F16, Q4])
+def test_tiles_of_very_different_scores(new, q4):
+    """Keys' scores in steps of 40 from tile to tile, up and down, the high ones of value zero but for one in a few: sums that grow
+    and shrink by e^40 again and again, and a row that sees only the low tiles."""
+    n, width = 1500, 64
+    rng, b, kp, vp, q = make_attention(("steps", new[0], int(q4)), q4, width, 64, 2, 1, new, [n, 60], spread=1.0)
+    for order in range(3):
+        keys, values = f32(rng, *kp.values().shape), f32(rng, *vp.values().shape)
+        level = np.arange(-(-n // 32))
+        level = [level % 2, level * 5 % 7, (level == 20) * 6][order]
+        for j in range(n):
+            pg, slot = b.place(0, j)
+            keys[pg, :, slot, 0] = level[j // 32]
+            if level[j // 32] and order != 1:
+                values[pg, :, slot] = 0
+        keys[..., 0] *= 8
+        kp.set(keys)
+        vp.set(values)
+        q[..., 0] = 40 * np.sqrt(width) / 8
+        want = R.attention(b, kp.values(), vp.values(), q, 1, 0.125)
+        # (where the high tiles' values are zero the rows' outputs are e^-40 and e^-240 of a value: 32-bit scores of up to 240 have
+        # errors of 2^-24 240 in the weights, and the scores' differences across tiles are rounded at up to 350)
+        bound = R.attention_bound(width, 1.0) + 2 * 2.0 ** -24 * 350
+        for hint in ((max(new), n), (max(new), 1)):
+            got, _ = run_attention(b, kp, vp, q, 1, longest=hint)
+            g, w = got[:new[0]].astype(np.float64), want[:new[0]]
+            if order == 2:  # all of the weight is the high tile's, and its values are zeros
+                assert np.abs(g).max() <= 2.0 ** -100
+                continue
+            assert norm_error(g, w) <= bound, (order, hint, norm_error(g, w), bound)
