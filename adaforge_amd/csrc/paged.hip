@@ -383,8 +383,8 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
 // pairs of keys are made by byte permutes.  A half of a tile lies in one page (pages hold at least 16 tokens), so its
 // base address is scalar and every load adds a constant per lane.
 //
-// fp32 rows enter as fp16 pairs hi + lo (22 bits and more): queries scaled by a power of two to below 32,
-// weights by one that the exponent takes in (Softmax).
+// fp32 rows enter as fp16 pairs hi + lo: queries scaled by a power of two (pair_scale), weights by one that the exponent takes
+// in (Softmax).
 
 constexpr int kPartSC1 = 16;      // buffer access policy sc1: through to (or from) the memory side
 constexpr int kWaitVm0 = 0x0F70;  // s_waitcnt vmcnt(0), expcnt and lgkmcnt unconstrained
@@ -418,6 +418,13 @@ __device__ __forceinline__ float less_half(float x, uint32_t h) {
     else
         asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
     return r;
+}
+
+// The power of two that brings a query whose largest element is mx to 2^14 .. 2^15: a pair then has 22 bits of every element down to
+// 2^-17 of the largest, and 2^-40 of that of smaller ones (one channel 1e5 times the others where the keys are zero: 4e-7
+// of the output wrong, with the largest below 32 8e-5).  At most 2^126, so that it and its reciprocal are finite.
+__device__ __forceinline__ float pair_scale(float mx) {
+    return mx > 0.0f ? ldexpf(1.0f, min(14 - ilogbf(mx), 126)) : 1.0f;
 }
 
 // The step and lane group whose operand holds channels 8 o .. 8 o + 7 of a key's row.
@@ -898,7 +905,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
 #pragma unroll
                 for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
             }
-            const float up = query_scale(row_max(mx));
+            const float up = pair_scale(row_max(mx));
             if (c < W / 8)
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -1338,7 +1345,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_ma
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[e]));
             }
-        const float up = query_scale(lanes4_max(mx));
+        const float up = pair_scale(lanes4_max(mx));
         qs = a.scale / up * kLog2e;
 #pragma unroll
         for (int st = 0; st < ST; ++st)

@@ -165,3 +165,25 @@ def test_tiles_of_very_different_scores(new, q4):
                 assert np.abs(g).max() <= 2.0 ** -100
                 continue
             assert norm_error(g, w) <= bound, (order, hint, norm_error(g, w), bound)
+
+
+# ---- query channels far apart in size -------------------------------------------------------------------
+
+@pytest.mark.parametrize("times", [1e3, 1e5, 3e6])
+@pytest.mark.parametrize("q4,width", [(F16, 64), (Q4, 64), (F16, 256), (Q4, 512)])
+@pytest.mark.parametrize("new", [FEW, MANY])
+def test_a_query_channel_far_above_the_others(new, q4, width, times):
+    """One channel many times the others, where the keys are zero: the scores are the others' and keep their digits.
+
+    Bound: that of 32-bit arithmetic, and for the small channels of a query, held to 2^-40 of its largest (errors uniform), what they
+    add to a score: 3 times 2^-40 / sqrt(3) times the largest, over scores of 2."""
+    rng, b, kp, vp, q = make_attention(("outlier", int(q4), width, new[0]), q4, width, 16, 2, 1, new, [700, 60])
+    keys = f32(rng, *kp.values().shape)
+    keys[..., 5] = 0
+    kp.set(keys)
+    assert (kp.values()[..., 5] == 0).all()
+    q[..., 5] = times * 2
+    want = R.attention(b, kp.values(), vp.values(), q, 1, 1 / np.sqrt(width))
+    got, _ = run_attention(b, kp, vp, q, 1)
+    bound = R.attention_bound(width, 2.0) + 3 * 2.0 ** -40 / np.sqrt(3) * times * 2
+    assert norm_error(got, want) <= bound, (norm_error(got, want), bound)
