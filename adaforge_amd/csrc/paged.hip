@@ -343,7 +343,10 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
             l = fmaf(l, al, lane == (j & 63) ? p : 0.0f);
             row(a.v_pages + off, slot, v);
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = p > 0.0f || p != p ? fmaf(p, v[e], acc[e] * al) : acc[e] * al;
+            for (int e = 0; e < E; ++e) {  // (no infinity times a weight of 0)
+                const float kept = al != 0.0f ? acc[e] * al : 0.0f;
+                acc[e] = p > 0.0f || p != p ? fmaf(p, v[e], kept) : kept;
+            }
             m = mn;
             if (p != p) {  // every output is a NaN
                 m = 0.0f;

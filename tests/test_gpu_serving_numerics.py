@@ -187,3 +187,28 @@ def test_a_query_channel_far_above_the_others(new, q4, width, times):
     got, _ = run_attention(b, kp, vp, q, 1)
     bound = R.attention_bound(width, 2.0) + 3 * 2.0 ** -40 / np.sqrt(3) * times * 2
     assert norm_error(got, want) <= bound, (norm_error(got, want), bound)
+
+
+# ---- infinite values that later keys outweigh --------------------------------------------------------------
+
+@pytest.mark.parametrize("new", [FEW, MANY])
+@pytest.mark.parametrize("at,above", [(3, 40), (3, 140), (3, 500), (600, 700)])
+def test_an_infinite_value_without_weight(new, at, above):
+    """An infinite value of a key that another outweighs by e^1000: it has no weight in 64 bits either, and the output is finite,
+    whether one wave or block takes both keys or not."""
+    n, width = 1000, 64
+    rng, b, kp, vp, q = make_attention(("outweighed", new[0], at), F16, width, 64, 2, 1, new, [n, 60], spread=1.0)
+    keys = f32(rng, *kp.values().shape)
+    keys[..., 0] = 0
+    pg, slot = b.place(0, above)
+    keys[pg, :, slot, 0] = 8
+    kp.set(keys)
+    pg, slot = b.place(0, at)
+    vp.planes()[0][pg, 0, slot, 7] = np.inf
+    q[..., 0] = 1000
+    want = R.attention(b, kp.values(), vp.values(), q, 1, 0.125)
+    assert np.isfinite(want).all()
+    for hint in ((max(new), n), (max(new), 1)):
+        got, _ = run_attention(b, kp, vp, q, 1, longest=hint)
+        assert np.isfinite(got).all(), hint
+        assert norm_error(got, want) <= R.attention_bound(width, 1.0) + 2.0 ** -23 * 1000
