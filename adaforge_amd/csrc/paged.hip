@@ -736,12 +736,19 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, const float* part
     }
 }
 
-// The chunks of a unit meet at its ticket: whether this block's, whose partial sums are stored, is the last one in.
+// The chunks of a unit meet at its ticket: whether this block's, whose partial sums are stored, is the last one in.  Where starts
+// fall, units of several sequences may be one, with different numbers of chunks: no block of such a launch draws, so that
+// every ticket is zero for the next (the starts are on their way while the sums are stored).
 __device__ __forceinline__ bool last_chunk(const PagedAttn& a, uint32_t unit, uint32_t parts) {
     __shared__ uint32_t last;
+    bool falls = false;
+    if (wave_id() == 0)
+        for (uint32_t i = threadIdx.x; i < a.b.sequences; i += 64) falls |= *gp(a.b.starts + i + 1) < *gp(a.b.starts + i);
+    const bool draws = !__any(falls);
     __builtin_amdgcn_s_waitcnt(kWaitVm0);
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0) last = 0;
+    if (threadIdx.x == 0 && draws) {
         uint32_t* t = a.tickets + unit * a.ticket_stride;
         last = __hip_atomic_fetch_add(t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
         if (last) __hip_atomic_store(t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

@@ -243,8 +243,8 @@ size_t af_kv_page_bytes(uint32_t type, uint32_t page, uint32_t kv_heads, uint32_
  * every access in bounds whatever they hold.  A position without a page (a table entry that is not below
  * `pages`, a position at or past table_stride * page, a negative one where lengths[s] is less than the sequence's
  * rows) is not written and not seen, and reads as zeros; rows at or past starts[sequences] are left as they were.
- * starts rises from 0 to at most `tokens` (later rows of a larger start are cut off); where it does not, rows and the
- * workspace of the call may hold anything afterwards. */
+ * starts rises from 0 to at most `tokens` (later rows of a larger start are cut off); where it does not, the rows of the
+ * call may hold anything afterwards (its workspace serves the next call). */
 typedef struct {
     const uint32_t* starts;  /* device [sequences + 1] */
     const uint32_t* lengths; /* device [sequences]: positions cached, the batch's included */
