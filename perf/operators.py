@@ -224,7 +224,7 @@ def _bind(s):
     from adaforge_amd import _native as N
     case, lib = s["case"], N.lib()
     p = lambda n: s[n].data_ptr()  # noqa: E731
-    s["native"], s["stream"] = N, torch.cuda.current_stream().cuda_stream
+    s["native"] = N
     size = N.sz()
     if case["kind"] == "select":
         a = N.LogitsArgs(p("logits"), case["vocabulary"], p("out"), case["vocabulary"], case["rows"], case["vocabulary"],
@@ -259,19 +259,19 @@ def _bind(s):
 
 def _run_own(s):
     N, case, kind = s["native"], s["case"], s["case"]["kind"]
-    lib = N.lib()
+    lib, stream = N.lib(), torch.cuda.current_stream().cuda_stream
     if kind == "select":
-        N.check(lib.af_logits_select(ctypes.byref(s["args"]), s["stream"]))
+        N.check(lib.af_logits_select(ctypes.byref(s["args"]), stream))
         return {"logits": s["out"], "result": s["result"]}
     if kind == "attend":
-        N.check(lib.af_paged_attention(ctypes.byref(s["args"]), s["stream"]))
+        N.check(lib.af_paged_attention(ctypes.byref(s["args"]), stream))
         return s["out"]
-    N.check(lib.af_kv_append(ctypes.byref(s["args"]), s["stream"]))
+    N.check(lib.af_kv_append(ctypes.byref(s["args"]), stream))
     if case["cache"] == "f16":
         return {"q": s["q_out"], "k": s["k_pages"], "v": s["v_pages"]}
     k, v = s["values"]
     a = s["args"]
-    N.check(lib.af_kv_read(ctypes.byref(a.pages), ctypes.byref(a.batch), k.data_ptr(), v.data_ptr(), s["stream"]))
+    N.check(lib.af_kv_read(ctypes.byref(a.pages), ctypes.byref(a.batch), k.data_ptr(), v.data_ptr(), stream))
     return {"q": s["q_out"], "k": k, "v": v}
 
 
