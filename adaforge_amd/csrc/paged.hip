@@ -290,14 +290,14 @@ constexpr float kLog2e = 1.44269504088896340736f, kLog2eLow = 1.9259629911266174
 
 // ---- attention, key by key ----------------------------------------------------------------------------
 
-// Softmax attention of one query by one wave, key by key in fp32 over key tiles t0, t0 + step, .. below t1 of T keys:
+// Softmax attention of one query by one wave, key by key in fp32 over key tiles t0, t0 + step, .. below t1:
 // values are read only where the query sees them.  What the products below fall back to where a sum of theirs is
 // not finite: there an infinite cached value meets halves of a pair that are zero or of the other sign, also
 // of keys that the row does not see; and where scores are so large that fp32 holds them to no less than parts of a unit (far_off).
 // Lane: channels E lane .. E lane + E - 1 (E = W / 64).  The sums are left as the products hold theirs, times 2^-m for a whole m (the
 // nearest to the maximum in base 2, whose remainder goes into them: maxima of 2^30, held to 128, would else join
 // as equals).
-template <int W, bool Q4, uint32_t T>
+template <int W, bool Q4>
 __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles, uint32_t t0, uint32_t t1, uint32_t step,
                                           uint32_t seq, uint32_t h, int32_t pos, uint32_t end, const float (&q)[W / 64],
                                           float (&acc)[W / 64], float& m, float& l) {
@@ -325,9 +325,9 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
     l = 0.0f;
 #pragma unroll 1
     for (uint32_t t = t0; t < t1; t += step) {
-        const uint32_t j0 = tile_at(tiles, t) * T;
+        const uint32_t j0 = tile_at(tiles, t) * 32;
 #pragma unroll 1
-        for (uint32_t j = j0; j < min(j0 + T, end); ++j) {
+        for (uint32_t j = j0; j < min(j0 + 32, end); ++j) {
             if (!sees(pos, (int32_t)j, a.window, a.sinks)) continue;
             const uint32_t page = page_of(a.b, seq, (int32_t)j);
             if (page >= a.b.pages) continue;
@@ -1049,7 +1049,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : 2) void paged_few_kernel(PagedA
                 const float* src = a.q + (size_t)(s.first + row / a.group) * a.q_stride + (size_t)(h * a.group + row % a.group) * W;
 #pragma unroll
                 for (int e = 0; e < E; ++e) q[e] = src[E * lane + e];
-                plain_row<W, Q4, 32>(a, keys, t0, t1, 4, seq, h, s.pos0 + (int32_t)(row / a.group), s.end, q, o, pm, pl2);
+                plain_row<W, Q4>(a, keys, t0, t1, 4, seq, h, s.pos0 + (int32_t)(row / a.group), s.end, q, o, pm, pl2);
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int e = 0; e < E; ++e) sums[(wave * HALFROWS + c - r0) * ROW + skewed(E * lane + e)] = o[e];
@@ -1559,7 +1559,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_ma
         const size_t at = (size_t)(h * a.group + r % a.group) * W + EL * lane, token = s.first + r / a.group;
 #pragma unroll
         for (int e = 0; e < EL; ++e) q[e] = a.q[token * a.q_stride + at + e];
-        plain_row<W, Q4, 32>(a, keys, t0, t1, 1, seq, h, s.pos0 + (int32_t)(r / a.group), s.end, q, o, pm, pl);
+        plain_row<W, Q4>(a, keys, t0, t1, 1, seq, h, s.pos0 + (int32_t)(r / a.group), s.end, q, o, pm, pl);
         float* dst = parts == 1 ? a.out + token * a.out_stride + at : part + (r - rt * R) * (W + 4) + EL * lane;
 #pragma unroll
         for (int e = 0; e < EL; ++e) dst[e] = parts > 1 ? o[e] : pl == 0.0f ? 0.0f : o[e] / pl;
