@@ -39,10 +39,11 @@ def test_a_pass_runs_on_the_stream_current_at_its_call(monkeypatch, case, names)
     args = type("Args", (ctypes.Structure,), {"_fields_": [("pages", inner), ("batch", inner)]})()
     t = torch.zeros(1)
     notes = Notes()
-    state = {"case": case, "native": notes, "stream": 1, "args": args, "values": [t, t],
+    state = {"case": case, "native": notes, "device": 0, "args": args, "values": [t, t],
              **{n: t for n in ("q", "k", "v", "q_out", "out", "k_pages", "v_pages", "result")}}
     for stream in (11, 12):
-        monkeypatch.setattr(torch.cuda, "current_stream", lambda s=stream: SimpleNamespace(cuda_stream=s))
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda *_, s=stream: SimpleNamespace(cuda_stream=s))
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda _, s=stream: s, raising=False)
         notes.calls.clear()
         cases.run(state)
         assert notes.calls == [(n, stream) for n in names]
