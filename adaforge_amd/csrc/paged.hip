@@ -373,14 +373,14 @@ __device__ __forceinline__ void plain_row(const PagedAttn& a, const Tiles& tiles
 // A block takes 16 of them against a chunk of the sequence's key tiles, its four waves tile by tile in turn; the
 // chunks of one row tile meet at a ticket, where the last block joins their partial sums (one pass over the
 // data with a running maximum and sum).  Bound by reading K and V once: one token at 32,768 positions (8 heads of 256,
-// fp16, 268 MB) 50.6 us = 5.3 TB/s, 32 of 1 to 8,192 positions 204 us = 5.3 TB/s; 4-bit rows by unpacking them (13
+// fp16, 268 MB) 50.2 us = 5.3 TB/s, 32 of 1 to 8,192 positions 194 us = 5.5 TB/s; 4-bit rows by unpacking them (13
 // instructions a word of eight) and by the waits between dependent steps: 64 windows of 1,024 41.8 us = 3.6 TB/s, eight
 // 512-wide heads of up to 32,768 positions (a block a CU) 35 us and 7 the join; short contexts by the chain of the
-// sequence's place, the page numbers, K, V, the ticket and the join: one token at 512 positions 10.6 us.
+// sequence's place, the page numbers, K, V, the ticket and the join: one token at 512 positions 10.4 us.
 //
 // Products are taken transposed on the fp16 matrix cores, S^T = K Q^T and O^T = V^T P^T (16 keys or channels by 16
-// rows): a lane holds one row's column throughout (row lane % 16), so the softmax needs two lane swaps per
-// tile and P is the second product's operand as it stands.  The order of the channels in the first sum and of the
+// rows): a lane holds one row's column throughout (row lane % 16), so the softmax needs lane swaps only
+// where its reference moves, and P is the second product's operand as it stands.  The order of the channels in the first sum and of the
 // keys in the second is free: lane group g = lane / 16 takes the channels its own 16-byte loads bring, and keys
 // 4 g .. 4 g + 3 of each half of a tile, so that K and V go from memory to operands in registers without LDS; V's
 // pairs of keys are made by byte permutes.  A half of a tile lies in one page (pages hold at least 16 tokens), so its
@@ -1400,7 +1400,7 @@ __global__ __launch_bounds__(256, W == 512 ? 1 : W >= 128 ? 2 : 4) void paged_ma
         }
     };
     f4 sv[2];
-    // the scores of tile `now`: masked where not every row sees every key, and taken into the running maximum
+    // the scores of tile `now`: masked where not every row sees every key, the softmax's reference brought along
     auto enter = [&] {
         if (!((now.ok == 3) & (now.j0 + 31 <= hi_one) & ((now.j0 >= lo_one) | (now.j0 + 31 < first))))
 #pragma unroll

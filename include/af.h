@@ -291,8 +291,11 @@ int af_kv_read(const af_kv_pages* pages, const af_kv_batch* batch, uint16_t* k, 
  * position p sees every key j <= p of its sequence with window == 0, j > p - window, or j < sinks (the first
  * tokens that stay visible).  out = softmax(scale q.k) v per query head (q_heads / kv_heads of them share a KV
  * head), zeros where nothing is seen.  q as af_kv_append writes it; q and out rows are [q_heads][width] floats,
- * strides and alignment as there, no row of out overlapping one of q.  fp32 softmax and sums; the queries and probabilities enter
- * the products with at least 22 significant bits.  longest_query (new tokens) and longest_context (length) of any
+ * strides and alignment as there, no row of out overlapping one of q.  fp32 scores (one past fp32's range counts as infinite),
+ * softmax and sums.  The queries and weights enter the products as two fp16 numbers each: a query's channel is held to 2^-23 of
+ * itself or 2^-40 of the row's largest, a weight to 2^-23 of itself or 2^-25 of the largest among its 32 neighbours (keys 32 i ..
+ * 32 i + 31), whichever is more; rows of base-2 scores beyond 2^21, or with infinities or NaNs, are taken key by key in fp32, right
+ * but many times slower.  longest_query (new tokens) and longest_context (length) of any
  * sequence are hints that only the split of the work, and the workspace's size, depend on: results are right
  * whatever they are, but one sequence may get slow where they are too small. */
 typedef struct {
