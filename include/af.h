@@ -295,7 +295,7 @@ int af_kv_read(const af_kv_pages* pages, const af_kv_batch* batch, uint16_t* k, 
  * softmax and sums.  The queries and weights enter the products as two fp16 numbers each: a query's channel is held to 2^-23 of
  * itself or 2^-40 of the row's largest, a weight to 2^-23 of itself or 2^-25 of the largest among its 32 neighbours (keys 32 i ..
  * 32 i + 31), whichever is more; rows of base-2 scores beyond 2^21, or with infinities or NaNs, are taken key by key in fp32, right
- * but many times slower.  longest_query (new tokens) and longest_context (length) of any
+ * but up to 60 times slower.  longest_query (new tokens) and longest_context (length) of any
  * sequence are hints that only the split of the work, and the workspace's size, depend on: results are right
  * whatever they are, but one sequence may get slow where they are too small. */
 typedef struct {
